@@ -378,6 +378,98 @@ int mxq_mx_linear_static(const void *x, int in_dtype, const uint8_t *w_codes, co
                          const void *bias, int out_dtype, int bias_dtype, int64_t M, int64_t N, int64_t K, int E, int F,
                          const uint8_t *floor_tab_host, int *status, const mxq_gemm_options *options, void *stream);
 
+/*
+ * Paged key/value cache in MX formats and the operators on it.  The reference quantizes cached keys and values as dense
+ * tensors (kv_cache_mxfp / kv_cache_mxint, chop/nn/quantized/functional/kvcache.py:8-43) and keeps them at full width;
+ * here the cache holds the codes and shared exponents themselves, in pages that sequences share out between them.
+ *
+ * Pages, one row of head_dim elements per (page, head, slot), contiguous, 16-byte aligned:
+ *   key, value                [pages, heads, page_size, row bytes]
+ *   key_scales, value_scales  uint8 [pages, heads, page_size, head_dim / 32] (NULL for MXQ_CACHE_BF16)
+ * Row formats (head_dim = D):
+ *   MXQ_CACHE_BF16     D bf16 values
+ *   MXQ_CACHE_E4M3     D MXFP codes sign | exponent | fraction (the bytes of mxq_mxfp_extract), E8M0 scales
+ *   MXQ_CACHE_E5M2     the same with 5 exponent and 2 fraction bits
+ *   MXQ_CACHE_E2M1X2   D/2 bytes, MXFP4 codes, element 2i in the low nibble of byte i
+ *   MXQ_CACHE_INT8     D int8 MXINT mantissas of `bits` bits (mxq_mxint_extract), biased shared exponents
+ * Token i of sequence b lives in slot i % page_size of page page_table[b * table_stride + i / page_size].
+ *
+ * Page tables and lengths are device memory and are only looked at on the device, so a captured launch follows their
+ * contents.  An entry that is needed and lies outside [0, pages), a length that is negative or does not fit the table
+ * (or the statistics given with it): the kernels store 8 in `status` (optional device int) and treat the page as absent
+ * (nothing is read from or written to it) or the length as the nearest valid one.
+ */
+#define MXQ_CACHE_BF16 0
+#define MXQ_CACHE_E4M3 1
+#define MXQ_CACHE_E5M2 2
+#define MXQ_CACHE_E2M1X2 3
+#define MXQ_CACHE_INT8 4
+
+typedef struct mxq_paged_cache {
+  void *key, *value;
+  uint8_t *key_scales, *value_scales;
+  int64_t pages;
+  int32_t format;    /* MXQ_CACHE_* */
+  int32_t bits;      /* MXQ_CACHE_INT8: mantissa bits, 2..8 */
+  int32_t heads;     /* key/value heads */
+  int32_t head_dim;  /* 32, 64, 128 or 256 */
+  int32_t page_size; /* 16, 32, 64, 128 or 256 */
+  int32_t reserved;  /* 0 */
+} mxq_paged_cache;
+
+/* sizeof(mxq_paged_cache) as the library was built, for bindings that mirror the struct by hand. */
+int mxq_paged_cache_size(void);
+
+/* Quantizes new keys and values into the pages: token t < counts[b] (counts NULL: t < tokens) of key / value
+ * [batch, heads, tokens, head_dim] goes to slot lengths[b] + t of sequence b, with the codes and shared exponents of
+ * the plain quantizers.  Element strides (batch, head, token); the last dimension is contiguous and every row starts on
+ * a 16-byte boundary.  positions (optional, int32 [batch, heads, positions_width] contiguous): the entry of every written
+ * slot becomes next_position[b] + t (next_position NULL: lengths[b] + t).  log2_tab_host: the floor table (MXFP) or the
+ * ceil table of `dtype` (MXINT); unused for MXQ_CACHE_BF16. */
+int mxq_paged_append(const mxq_paged_cache *cache, const void *key, const void *value, int dtype, int64_t batch,
+                     int64_t tokens, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t, int64_t v_stride_b,
+                     int64_t v_stride_h, int64_t v_stride_t, const int32_t *page_table, int64_t table_width,
+                     int64_t table_stride, const int32_t *lengths, const int32_t *counts, int32_t *positions,
+                     int64_t positions_width, const int32_t *next_position, const uint8_t *log2_tab_host, int *status,
+                     void *stream);
+
+/* The cached rows as dense tensors: key, value [batch, heads, max_tokens, head_dim] of `dtype`, contiguous; rows from
+ * lengths[b] on are zeros. */
+int mxq_paged_gather(const mxq_paged_cache *cache, void *key, void *value, int dtype, int64_t batch, int64_t max_tokens,
+                     const int32_t *page_table, int64_t table_width, int64_t table_stride, const int32_t *lengths,
+                     int *status, void *stream);
+
+/* Attention of one new token per sequence over the pages, split over the cache's length and joined:
+ *   s_j = scaling * <q, k_j>,  out = sum_j softmax(s)_j v_j  over j < lengths[b]  (zeros for an empty sequence)
+ * q, out: [batch, q_heads, head_dim] of `dtype`; q with element strides (batch, head) and a contiguous last dimension, out
+ * contiguous.  q_heads is a multiple of heads: query heads h * g .. h * g + g - 1 read key/value head h.
+ * weights (optional, fp32 [batch, heads, weights_width] contiguous): weights[b, h, j] += sum of softmax(s)_j over the
+ * query heads of h.  workspace: 16-byte aligned, at least mxq_paged_attention_workspace_bytes(...) bytes, not shared with
+ * a call that may run at the same time. */
+int64_t mxq_paged_attention_workspace_bytes(const mxq_paged_cache *cache, int64_t batch, int64_t q_heads,
+                                            int64_t table_width, int with_weights);
+int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, int dtype, int64_t batch, int64_t q_heads,
+                        int64_t q_stride_b, int64_t q_stride_h, float scaling, const int32_t *page_table,
+                        int64_t table_width, int64_t table_stride, const int32_t *lengths, float *weights,
+                        int64_t weights_width, void *workspace, int64_t workspace_bytes, int *status, void *stream);
+
+/* Eviction by accumulated attention weight, in place, per sequence and key/value head.  A sequence of more than `keep`
+ * tokens keeps `keep` of them: first those whose position is at least next_position[b] - recent, then those with the
+ * largest weight, the lowest slot first among equals (a NaN weight ranks below every other).  The i-th free slot below
+ * `keep` takes the row of the i-th kept token at or above `keep`; rows that stay are not touched.
+ *   weights    fp32  [batch, heads, width]   in
+ *   positions  int32 [batch, heads, width]   in, or NULL: slot indices (with next_position ignored, lengths taken)
+ *   new_lengths int32 [batch] = min(lengths, keep); new_weights, new_positions [batch, heads, width]: the statistics of
+ *   the new slots, 0 and -1 from the new length on.  Not overlapping the inputs.
+ * The weights must be finite or NaN for the order above; page tables are not changed: the pages behind
+ * ceil(new length / page_size) are free. */
+int64_t mxq_paged_evict_workspace_bytes(const mxq_paged_cache *cache, int64_t batch, int64_t width, int64_t keep);
+int mxq_paged_evict(const mxq_paged_cache *cache, int64_t batch, const int32_t *page_table, int64_t table_width,
+                    int64_t table_stride, const int32_t *lengths, const float *weights, const int32_t *positions,
+                    const int32_t *next_position, int64_t width, int64_t keep, int64_t recent, int32_t *new_lengths,
+                    float *new_weights, int32_t *new_positions, void *workspace, int64_t workspace_bytes, int *status,
+                    void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -57,6 +57,18 @@ _PROTOTYPES = {
                              c_int64, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     "mxq_bfp_fake_tiles": [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int, c_int,
                            c_void_p, c_void_p],
+    "mxq_paged_cache_size": [],
+    "mxq_paged_append": [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+                         c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+                         c_void_p, c_void_p],
+    "mxq_paged_gather": [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p,
+                         c_void_p],
+    "mxq_paged_attention_workspace_bytes": [c_void_p, c_int64, c_int64, c_int64, c_int],
+    "mxq_paged_attention": [c_void_p, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64, c_int64, ctypes.c_float, c_void_p,
+                            c_int64, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p],
+    "mxq_paged_evict_workspace_bytes": [c_void_p, c_int64, c_int64, c_int64],
+    "mxq_paged_evict": [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
+                        c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_void_p, c_void_p],
     "mxq_bfp_fake": [c_void_p, c_void_p, c_int, c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p, c_void_p],
 }
 
@@ -69,9 +81,18 @@ class GemmOptions(ctypes.Structure):
                 ("no_transposed", ctypes.c_int32)]
 
 
+class PagedCache(ctypes.Structure):
+    """`mxq_paged_cache` of include/mxq.h: the pages of one key/value cache."""
+
+    _fields_ = [("key", c_void_p), ("value", c_void_p), ("key_scales", c_void_p), ("value_scales", c_void_p),
+                ("pages", ctypes.c_int64), ("format", ctypes.c_int32), ("bits", ctypes.c_int32), ("heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("page_size", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 TILES_AUTO, TILES_SINGLE, TILES_PAIRS = 0, 1, 2
 GEMM_STATIC_B, GEMM_A_E5M2 = 1, 4  # bits of GemmOptions.flags
 CODES_E4M3, CODES_E2M1X2, CODES_E5M2 = 0, 1, 2
+CACHE_BF16, CACHE_E4M3, CACHE_E5M2, CACHE_E2M1X2, CACHE_INT8 = 0, 1, 2, 3, 4
 TEST_DROP_LAST_LOAD = 1
 
 
@@ -105,6 +126,8 @@ def lib():
         handle.mxq_error_string.restype = c_char_p
         if handle.mxq_gemm_options_size() != ctypes.sizeof(GemmOptions):
             raise MxqError("mxq_gemm_options of libmxq.so and its ctypes mirror differ in size: rebuild the library")
+        if handle.mxq_paged_cache_size() != ctypes.sizeof(PagedCache):
+            raise MxqError("mxq_paged_cache of libmxq.so and its ctypes mirror differ in size: rebuild the library")
         _lib = handle
     return _lib
 

@@ -34,6 +34,7 @@ _STATUS_TEXT = {
     4: "epilogue: wait for a finished accumulator ran out",
     5: "CTA pair: the two CTAs got different tensor-memory addresses",
     7: "peer barrier: a GPU of the tensor-parallel group did not arrive within the wait limit",
+    8: "paged cache: a page table entry or a length points outside of the cache",
 }
 
 
@@ -112,7 +113,8 @@ def _status(device: torch.device) -> Tensor:
 
 
 def check_status(device=None) -> None:
-    """Synchronise and raise if a GEMM kernel on `device` reported that one of its bounded waits ran out."""
+    """Synchronise and raise if a kernel on `device` reported that one of its bounded waits ran out or that a page table
+    or length of a paged cache pointed outside of it."""
     devices = list(_STATUS) if device is None else [torch.device(device).index or 0]
     for idx in devices:
         t = _STATUS.get(idx)
@@ -121,7 +123,8 @@ def check_status(device=None) -> None:
         code = int(t.item())
         if code:
             t.zero_()
-            raise _lib.MxqError(f"GEMM kernel on cuda:{idx} gave up: {_STATUS_TEXT.get(code, code)}")
+            raise _lib.MxqError(f"{'kernel' if code == 8 else 'GEMM kernel'} on cuda:{idx} gave up: "
+                                f"{_STATUS_TEXT.get(code, code)}")
 
 
 def _bias_args(bias: Tensor | None):
