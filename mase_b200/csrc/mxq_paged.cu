@@ -453,7 +453,7 @@ int mxq_paged_append(const mxq_paged_cache *cache, const void *key, const void *
   int rc = read_cache(cache, c);
   if (rc != MXQ_OK) return rc;
   if (dtype != MXQ_F32 && dtype != MXQ_BF16) return MXQ_ERR_DTYPE;
-  if (batch < 0 || tokens < 0 || tokens > INT32_MAX || c.heads > 32767) return MXQ_ERR_SHAPE;
+  if (batch < 0 || tokens < 0 || tokens > INT32_MAX) return MXQ_ERR_SHAPE;
   if (batch == 0 || tokens == 0) return MXQ_OK;
   if ((rc = read_table(page_table, table_width, table_stride, batch, c.page_log2)) != MXQ_OK) return rc;
   if (!key || !value || !lengths || (!log2_tab_host && cache->format != MXQ_CACHE_BF16)) return MXQ_ERR_NULL;
@@ -494,7 +494,7 @@ int mxq_paged_gather(const mxq_paged_cache *cache, void *key, void *value, int d
   int rc = read_cache(cache, c);
   if (rc != MXQ_OK) return rc;
   if (dtype != MXQ_F32 && dtype != MXQ_BF16) return MXQ_ERR_DTYPE;
-  if (batch < 0 || max_tokens < 0 || max_tokens > INT32_MAX || c.heads > 32767) return MXQ_ERR_SHAPE;
+  if (batch < 0 || max_tokens < 0 || max_tokens > INT32_MAX) return MXQ_ERR_SHAPE;
   if (batch == 0 || max_tokens == 0) return MXQ_OK;
   if ((rc = read_table(page_table, table_width, table_stride, batch, c.page_log2)) != MXQ_OK) return rc;
   if (!key || !value || !lengths) return MXQ_ERR_NULL;

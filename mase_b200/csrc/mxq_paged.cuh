@@ -40,7 +40,7 @@ inline int read_cache(const mxq_paged_cache *c, Cache &out) {
   if (c->format != MXQ_CACHE_BF16 && (!c->key_scales || !c->value_scales)) return MXQ_ERR_NULL;
   if (c->head_dim != 32 && c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return MXQ_ERR_UNSUPPORTED;
   if (c->page_size < 16 || c->page_size > 256 || (c->page_size & (c->page_size - 1))) return MXQ_ERR_UNSUPPORTED;
-  if (c->heads < 1 || c->heads > 65535 || c->pages < 0 || c->pages > INT32_MAX) return MXQ_ERR_SHAPE;
+  if (c->heads < 1 || c->heads > 32767 || c->pages < 0 || c->pages > INT32_MAX) return MXQ_ERR_SHAPE;
   if (!aligned(c->key, 16) || !aligned(c->value, 16) || !aligned(c->key_scales, 16) || !aligned(c->value_scales, 16))
     return MXQ_ERR_ALIGN;
   out.codes[0] = static_cast<uint8_t *>(c->key), out.codes[1] = static_cast<uint8_t *>(c->value);

@@ -29,22 +29,26 @@ namespace mxq {
 namespace paged {
 
 constexpr int kWarps = 4;
-constexpr int kTile = 16;
-constexpr int kJoinThreads = 128;
+constexpr int kTile = 16;                // cached tokens of a warp's tile
+constexpr int kUnit = kWarps * kTile;    // tokens that a CTA takes at a time: the grain of the split
+constexpr int kRowCost = 2;            // units that a row counts for beyond its tokens
+constexpr int kFinishThreads = 128;
 
 struct AttnArgs {
   const void *q;
   void *out;
   int64_t q_stride_b, q_stride_h;
-  float scaling;
-  int group;     // query heads per key/value head
+  float c_hi, c_lo;  // scaling * log2(e) in two terms
+  int group;       // query heads per key/value head
   int q_heads;
-  int head_tiles;
+  int head_tiles;  // tiles of 8 * NT query heads of a group
+  int batch;
   const int32_t *lengths;
-  int64_t most;  // tokens that tables (and weights) can hold
-  int chunk, chunks;
-  float *part_o;   // [batch, q_heads, chunks, dim]
-  float2 *part_ml; // [batch, q_heads, chunks]: maximum and sum
+  int64_t most;    // tokens that tables (and weights) can hold
+  int ctas;        // CTAs of the launch
+  float *part_o;   // [ctas, 2, 8 * NT, dim]: unnormalised results of the rows a CTA shares with others
+  float2 *part_ml; // [ctas, 2, 8 * NT]: their maximum and sum
+  float2 *stats;   // [batch, q_heads] maximum and sum of rows of one CTA, when weights are accumulated
   float *scores;   // [batch, heads, head_tiles, tokens, 8 * NT] when weights are accumulated
   int64_t score_tokens;
   float *weights;
@@ -63,7 +67,9 @@ __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-// exponent offset of the raw bf16 pattern of a code: value = raw * 2^offset * 2^(scale - 127)
+// The raw bf16 pattern of a code stands for raw = value * 2^-offset in units of the block scale, so a block's factor is
+// 2^(scale - 127 + offset), in bf16 the exponent field scale + offset.  That field is out of [1, 254] for MXFP blocks with
+// a scale far above one and for MXINT blocks at either end: those tiles take a second factor (kRare).
 template <int kFormat>
 __device__ __forceinline__ int raw_offset(int bits) {
   if constexpr (kFormat == MXQ_CACHE_INT8)
@@ -73,85 +79,113 @@ __device__ __forceinline__ int raw_offset(int bits) {
   else
     return 127 - ((1 << (Format<kFormat>::E - 1)) - 1);
 }
-// bf16 pattern of 2^x, x >= -133 (0 below); x above 127 saturates
-__device__ __forceinline__ uint32_t pow2_bf16(int x) {
-  if (x > 127) x = 127;
-  return x >= -126 ? (uint32_t)(x + 127) << 7 : (x >= -133 ? 1u << (x + 133) : 0u);
-}
-// The multiplier of a block; kBig: the part of the exponent above 127 goes into `rest`.
 template <int kFormat>
-__device__ __forceinline__ int block_exponent(uint32_t scale, int bits) {
-  if (kFormat == MXQ_CACHE_INT8 && scale == 255) return 128;  // 2^128: the reference multiplies zeros by inf
-  return (int)scale - 127 + raw_offset<kFormat>(bits);
+__device__ __forceinline__ bool rare_scale(uint32_t scale, int offset) {
+  if constexpr (kFormat == MXQ_CACHE_INT8)
+    return (int)scale + offset < 1 || scale == 255u;
+  else
+    return (int)scale + offset > 254;
+}
+// first factor of a rare block (bf16 pattern): the field clamped to 254; for MXINT also subnormal powers, and infinity
+// for scale byte 255 (the reference multiplies the zero mantissas of such a block by 2^128)
+template <int kFormat>
+__device__ __forceinline__ uint32_t rare_factor(uint32_t scale, int offset) {
+  const int field = (int)scale + offset;
+  if constexpr (kFormat == MXQ_CACHE_INT8) {
+    if (scale == 255u) return 0x7F80u;
+    return field >= 1 ? (uint32_t)field << 7 : (field > -7 ? 1u << (field + 6) : 0u);
+  }
+  return (uint32_t)min(field, 254) << 7;
 }
 template <int kFormat>
-__device__ __forceinline__ uint32_t block_factor(int x) {
-  if (kFormat == MXQ_CACHE_INT8 && x == 128) return 0x7F80u;
-  return pow2_bf16(x);
+__device__ __forceinline__ uint32_t rare_rest(uint32_t scale, int offset) {
+  return (uint32_t)(127 + max((int)scale + offset - 254, 0)) << 7;
 }
 
-// Two codes, one in the upper byte of each half of x (what is in the lower bytes does not matter) -> raw bf16 pair.
+template <bool kRare>
+__device__ __forceinline__ uint32_t scaled(uint32_t raw, uint32_t f, uint32_t rest) {
+  raw = mul2(raw, f);
+  return kRare ? mul2(raw, rest) : raw;
+}
+
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {  // one instruction
+  uint32_t d;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "r"(mask), "r"(bits));
+  return d;
+}
+// Four 8-bit codes -> upper and lower bytes of their raw bf16 patterns: sign, then exponent and fraction fields moved down
+// to the bf16 fraction boundary.
 template <int kFormat>
-__device__ __forceinline__ uint32_t raw_upper(uint32_t x) {
-  if constexpr (kFormat == MXQ_CACHE_E4M3) return ((x >> 4) & 0x07F007F0u) | (x & 0x80008000u);
-  if constexpr (kFormat == MXQ_CACHE_E5M2) return ((x >> 3) & 0x0FE00FE0u) | (x & 0x80008000u);
-  return 0;
+__device__ __forceinline__ void split_bytes(uint32_t w, uint32_t &hi, uint32_t &lo) {
+  if constexpr (kFormat == MXQ_CACHE_E4M3) {
+    hi = and_or(w, 0x80808080u, (w >> 4) & 0x07070707u), lo = (w << 4) & 0xF0F0F0F0u;
+  } else {
+    hi = and_or(w, 0x80808080u, (w >> 3) & 0x0F0F0F0Fu), lo = (w << 5) & 0xE0E0E0E0u;
+  }
+}
+// Eight E2M1 codes -> the same bytes of the even (0, 2, 4, 6) and odd (1, 3, 5, 7) ones.
+__device__ __forceinline__ void split_nibbles(uint32_t w, uint32_t &hi_even, uint32_t &lo_even, uint32_t &hi_odd,
+                                              uint32_t &lo_odd) {
+  hi_even = and_or(w << 4, 0x80808080u, (w >> 2) & 0x01010101u), lo_even = (w << 6) & 0xC0C0C0C0u;
+  hi_odd = and_or(w, 0x80808080u, (w >> 6) & 0x01010101u), lo_odd = (w << 2) & 0xC0C0C0C0u;
 }
 // Two int8, one in the lower byte of each half -> bf16 pair: 128 + (u & 127) minus 128 or 256 by the sign bit.
 __device__ __forceinline__ uint32_t int8_lower(uint32_t x) {
-  return sub2((x & 0x007F007Fu) | 0x43004300u, (x & 0x00800080u) | 0x43004300u);
-}
-// Nibble i (0..3) of each half -> raw bf16 pair of E2M1.
-template <int i>
-__device__ __forceinline__ uint32_t raw_nibble(uint32_t x) {
-  if constexpr (i == 0) return ((x << 12) & 0x80008000u) | ((x << 6) & 0x01C001C0u);
-  if constexpr (i == 1) return ((x << 8) & 0x80008000u) | ((x << 2) & 0x01C001C0u);
-  if constexpr (i == 2) return ((x << 4) & 0x80008000u) | ((x >> 2) & 0x01C001C0u);
-  return (x & 0x80008000u) | ((x >> 6) & 0x01C001C0u);
+  return sub2(and_or(x, 0x007F007Fu, 0x43004300u), and_or(x, 0x00800080u, 0x43004300u));
 }
 
-template <bool kBig>
-__device__ __forceinline__ uint32_t scaled(uint32_t raw, uint32_t f, uint32_t rest) {
-  raw = mul2(raw, f);
-  return kBig ? mul2(raw, rest) : raw;
+// One word of a key row -> bf16 pairs.  Halves of pair i of the word are these elements, from the word's first one:
+//   16 bit: 0, 1;  E4M3 / E5M2: 2 i, 2 i + 1;  int8: i, i + 2;  E2M1: 4 (i & 1) + (i >> 1) and that + 2
+template <int kFormat>
+__device__ __forceinline__ int pair_element(int i, int half) {
+  if (kFormat == MXQ_CACHE_INT8) return i + 2 * half;
+  if (kFormat == MXQ_CACHE_E2M1X2) return 4 * (i & 1) + (i >> 1) + 2 * half;
+  return 2 * i + half;
 }
-
-// One word of a key row -> bf16 pairs.  Pair i of the word holds these elements (relative to the word's first one):
-//   16 bit: (0, 1);  8 bit: (i, i + 2);  4 bit: (i, i + 4)
-template <int kFormat, bool kBig>
+template <int kFormat, bool kRare>
 __device__ __forceinline__ void key_word(uint32_t w, uint32_t f, uint32_t rest, uint32_t *out) {
   if constexpr (kFormat == MXQ_CACHE_BF16) {
     out[0] = w;
   } else if constexpr (kFormat == MXQ_CACHE_INT8) {
-    out[0] = scaled<kBig>(int8_lower(w), f, rest), out[1] = scaled<kBig>(int8_lower(w >> 8), f, rest);
+    out[0] = scaled<kRare>(int8_lower(w), f, rest), out[1] = scaled<kRare>(int8_lower(w >> 8), f, rest);
   } else if constexpr (Format<kFormat>::kBits == 8) {
-    out[0] = scaled<kBig>(raw_upper<kFormat>(w << 8), f, rest), out[1] = scaled<kBig>(raw_upper<kFormat>(w), f, rest);
+    uint32_t hi, lo;
+    split_bytes<kFormat>(w, hi, lo);
+    out[0] = scaled<kRare>(__byte_perm(lo, hi, 0x5140), f, rest), out[1] = scaled<kRare>(__byte_perm(lo, hi, 0x7362), f, rest);
   } else {
-    out[0] = scaled<kBig>(raw_nibble<0>(w), f, rest), out[1] = scaled<kBig>(raw_nibble<1>(w), f, rest);
-    out[2] = scaled<kBig>(raw_nibble<2>(w), f, rest), out[3] = scaled<kBig>(raw_nibble<3>(w), f, rest);
+    uint32_t he, le, ho, lo;
+    split_nibbles(w, he, le, ho, lo);
+    out[0] = scaled<kRare>(__byte_perm(le, he, 0x5140), f, rest), out[1] = scaled<kRare>(__byte_perm(le, he, 0x7362), f, rest);
+    out[2] = scaled<kRare>(__byte_perm(lo, ho, 0x5140), f, rest), out[3] = scaled<kRare>(__byte_perm(lo, ho, 0x7362), f, rest);
   }
 }
 // The same word of two value rows -> pairs (row a, row b) of its elements 0, 1, 2, ...
-template <int kFormat, bool kBig>
+template <int kFormat, bool kRare>
 __device__ __forceinline__ void value_words(uint32_t a, uint32_t b, uint32_t f, uint32_t rest, uint32_t *out) {
   if constexpr (kFormat == MXQ_CACHE_BF16) {
     out[0] = __byte_perm(a, b, 0x5410), out[1] = __byte_perm(a, b, 0x7632);
   } else if constexpr (kFormat == MXQ_CACHE_INT8) {
-    out[0] = scaled<kBig>(int8_lower(__byte_perm(a, b, 0x4400)), f, rest);
-    out[1] = scaled<kBig>(int8_lower(__byte_perm(a, b, 0x5511)), f, rest);
-    out[2] = scaled<kBig>(int8_lower(__byte_perm(a, b, 0x6622)), f, rest);
-    out[3] = scaled<kBig>(int8_lower(__byte_perm(a, b, 0x7733)), f, rest);
-  } else if constexpr (Format<kFormat>::kBits == 8) {
-    out[0] = scaled<kBig>(raw_upper<kFormat>(__byte_perm(a, b, 0x4400)), f, rest);
-    out[1] = scaled<kBig>(raw_upper<kFormat>(__byte_perm(a, b, 0x5511)), f, rest);
-    out[2] = scaled<kBig>(raw_upper<kFormat>(__byte_perm(a, b, 0x6622)), f, rest);
-    out[3] = scaled<kBig>(raw_upper<kFormat>(__byte_perm(a, b, 0x7733)), f, rest);
+    out[0] = scaled<kRare>(int8_lower(__byte_perm(a, b, 0x4400)), f, rest);
+    out[1] = scaled<kRare>(int8_lower(__byte_perm(a, b, 0x5511)), f, rest);
+    out[2] = scaled<kRare>(int8_lower(__byte_perm(a, b, 0x6622)), f, rest);
+    out[3] = scaled<kRare>(int8_lower(__byte_perm(a, b, 0x7733)), f, rest);
   } else {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const uint32_t x = __byte_perm(a, b, h ? 0x7632 : 0x5410);
-      out[4 * h + 0] = scaled<kBig>(raw_nibble<0>(x), f, rest), out[4 * h + 1] = scaled<kBig>(raw_nibble<1>(x), f, rest);
-      out[4 * h + 2] = scaled<kBig>(raw_nibble<2>(x), f, rest), out[4 * h + 3] = scaled<kBig>(raw_nibble<3>(x), f, rest);
+      const uint32_t x = __byte_perm(a, b, h ? 0x7362 : 0x5140);  // bytes a, b, a, b of neighbouring positions
+      if constexpr (Format<kFormat>::kBits == 8) {
+        uint32_t hi, lo;
+        split_bytes<kFormat>(x, hi, lo);
+        out[2 * h] = scaled<kRare>(__byte_perm(lo, hi, 0x5140), f, rest);
+        out[2 * h + 1] = scaled<kRare>(__byte_perm(lo, hi, 0x7362), f, rest);
+      } else {
+        uint32_t he, le, ho, lo;
+        split_nibbles(x, he, le, ho, lo);
+        out[4 * h] = scaled<kRare>(__byte_perm(le, he, 0x5140), f, rest);
+        out[4 * h + 1] = scaled<kRare>(__byte_perm(lo, ho, 0x5140), f, rest);
+        out[4 * h + 2] = scaled<kRare>(__byte_perm(le, he, 0x7362), f, rest);
+        out[4 * h + 3] = scaled<kRare>(__byte_perm(lo, ho, 0x7362), f, rest);
+      }
     }
   }
 }
@@ -167,19 +201,33 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-// kBytes (2, 4, 8 or 16) contiguous bytes as words
+// ---- asynchronous copies into a warp's ring --------------------------------------------------------------------------
+template <int kBytes>
+__device__ __forceinline__ void copy_async(uint8_t *dst, const uint8_t *src) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  if constexpr (kBytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(d), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(d), "l"(src), "n"(kBytes) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+// kBytes (2, 4, 8 or 16) bytes of shared memory as words
 template <int kBytes>
 __device__ __forceinline__ void load_piece(const uint8_t *p, uint32_t *w) {
   if constexpr (kBytes == 16) {
-    const uint4 r = __ldcs(reinterpret_cast<const uint4 *>(p));
+    const uint4 r = *reinterpret_cast<const uint4 *>(p);
     w[0] = r.x, w[1] = r.y, w[2] = r.z, w[3] = r.w;
   } else if constexpr (kBytes == 8) {
-    const uint2 r = __ldcs(reinterpret_cast<const uint2 *>(p));
+    const uint2 r = *reinterpret_cast<const uint2 *>(p);
     w[0] = r.x, w[1] = r.y;
   } else if constexpr (kBytes == 4) {
-    w[0] = __ldcs(reinterpret_cast<const uint32_t *>(p));
+    w[0] = *reinterpret_cast<const uint32_t *>(p);
   } else {
-    w[0] = __ldcs(reinterpret_cast<const unsigned short *>(p));
+    w[0] = *reinterpret_cast<const uint16_t *>(p);
   }
 }
 
@@ -195,13 +243,32 @@ struct Shape {
   static constexpr int kValWords = (kValPiece + 3) / 4;
   static constexpr int kValElems = kValPiece * 8 / kBits;           // elements of a piece
   static constexpr int kPairs = kBits == 16 ? 1 : (kBits == 8 ? 2 : 4);  // bf16 pairs of a key word
+  static constexpr int kScaleRow = kFormat == MXQ_CACHE_BF16 ? 0 : D / 32;  // scale bytes of a row
+  // One stage of a warp's ring: the tile's key rows, its value rows, the scale bytes of both.  The rows of a tile are
+  // contiguous in their page and are copied in order, 512 bytes an instruction; where they land is permuted in units of
+  // 16 (keys) or 32 bytes inside each 128-byte line, so that the lanes' reads (below) hit every bank once.
+  static constexpr int kSide = kTile * kRow;
+  static constexpr int kScaleBytes = kTile * kScaleRow;
+  static constexpr int kStage = 2 * kSide + 2 * kScaleBytes;
+  // where byte `byte` of a token's row lies in the stage
+  static __device__ __forceinline__ int key_slot(int token, int byte) {
+    return token * kRow + byte ^ (kRow >= 128 ? (token & 1) << 6 : 0);
+  }
+  static __device__ __forceinline__ int value_slot(int token, int byte) {
+    return token * kRow + byte ^ (kRow >= 32 ? ((token >> 1) & 3) << 5 : 0);
+  }
+  // the parts of a slot's permutation that a copy at byte i (a multiple of 512) of the tile adds to that of byte 0
+  static __host__ __device__ constexpr int key_turn(int i) { return kRow == 512 ? ((i >> 9) & 1) << 6 : 0; }
+  static __host__ __device__ constexpr int value_turn(int i) {
+    return kRow == 128 ? ((i >> 8) & 3) << 5 : (kRow == 256 ? ((i >> 9) & 3) << 5 : (kRow == 512 ? ((i >> 10) & 3) << 5 : 0));
+  }
+  static constexpr int kStages = kRow <= 64 ? 4 : (kRow <= 128 ? 2 : 2);
 };
 // element (0 .. D-1) that half `half` of pair i of key word w of piece c of lane t holds
 template <int kFormat, int D>
 __device__ __forceinline__ int key_element(int c, int w, int i, int half, int t) {
   using S = Shape<kFormat, D>;
-  const int first = (c * 4 * S::kKeyPiece + t * S::kKeyPiece + w * 4) * 8 / S::kBits;
-  return first + (S::kBits == 16 ? half : (S::kBits == 8 ? i + 2 * half : i + 4 * half));
+  return (c * 4 * S::kKeyPiece + t * S::kKeyPiece + w * 4) * 8 / S::kBits + pair_element<kFormat>(i, half);
 }
 // element that entry e (0 .. D/8 - 1) of value lane r holds
 template <int kFormat, int D>
@@ -215,14 +282,22 @@ __device__ __forceinline__ float load_q(const __nv_bfloat16 *p) { return __bfloa
 __device__ __forceinline__ float load_q(const float *p) { return *p; }
 __device__ __forceinline__ float bf16_of(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
 
-constexpr float kLog2e = 1.4426950408889634f;
-// A tile raises the running maximum only when a score exceeds it by more than this: probabilities then stay below
-// e^8 and the rescaling (shuffles, D/4 products) runs a few times per warp instead of once per tile.
-constexpr float kSlack = 8.f;
+// Scores are kept in units of log2: x_j = scaling * log2(e) * <q, k_j>, and the softmax is 2^(x_j - m) / sum.
+// A tile raises the reference m only when a score exceeds it by more than kSlack: probabilities then stay below 2^11.5
+// and the rescaling (shuffles, D/4 products) runs a few times per warp instead of once per tile.
+constexpr float kSlack = 11.5f;
+constexpr float kLowest = -3.0e38f;  // m before the first score: finite, so that no difference is inf - inf
+
+__device__ __forceinline__ float exp2_fast(float x) {  // results below 2^-126 become 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 template <typename T, int kFormat, int D, int NT>
 struct Worker {
   using S = Shape<kFormat, D>;
+  int key_at[2], value_at[2];  // where the lane reads: key pieces of even and odd number, value rows 2t and 2t + 1
   static constexpr int kTerms = Elem<T>::kBf16 ? 1 : 3;   // bf16 terms of a query element
   static constexpr int kPTerms = Elem<T>::kBf16 ? 2 : 3;  // and of a probability
   static constexpr int kSteps = D / 16;
@@ -230,7 +305,15 @@ struct Worker {
   float o[kSteps][NT][4];
   float m[NT][2], l[NT][2];
 
-  __device__ __forceinline__ void start(const T *qrow, int64_t stride_h, int heads, int lane) {
+  __device__ __forceinline__ void setup(int lane) {
+    const int t = lane & 3, r = lane >> 2;
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      key_at[x] = S::key_slot(r, x * 64 + t * S::kKeyPiece);
+      value_at[x] = S::value_slot(2 * t + x, r * S::kValPiece);
+    }
+  }
+  __device__ __forceinline__ void load_query(const T *qrow, int64_t stride_h, int heads, int lane) {
     const int t = lane & 3, head = lane >> 2;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -249,24 +332,33 @@ struct Worker {
           v[0] -= bf16_of(v[0]), v[1] -= bf16_of(v[1]);
         }
       }
-#pragma unroll
-      for (int h = 0; h < 2; ++h) m[n][h] = -INFINITY, l[n][h] = 0.f;
     }
+  }
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-    for (int j = 0; j < kSteps; ++j)
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
+      for (int h = 0; h < 2; ++h) m[n][h] = kLowest, l[n][h] = 0.f;
+#pragma unroll
+      for (int j = 0; j < kSteps; ++j)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[j][n][i] = 0.f;
+    }
   }
 
-  // kk: key words of tokens r and r + 8; vv: value words of tokens 2t, 2t + 1, 2t + 8, 2t + 9; fk, fv: their exponents
-  template <bool kBig>
-  __device__ __forceinline__ void tile(const uint32_t (&kk)[2][S::kKeyPieces][S::kKeyWords],
-                                       const uint32_t (&vv)[4][S::kValPieces][S::kValWords],
-                                       const int (&xk)[2][S::kKeyPieces], const int (&xv)[4][S::kValPieces], int live,
-                                       float scaling, float *scores, int lane) {
+  // x - m in units of log2; fp32 queries take the factor scaling * log2(e) with 48 bits
+  static __device__ __forceinline__ float score(float s, float c_hi, float c_lo, float m) {
+    const float x = fmaf(s, c_hi, -m);
+    return Elem<T>::kBf16 ? x : fmaf(s, c_lo, x);
+  }
+
+  // One tile from a stage of the ring; `live` tokens of it exist.
+  template <bool kRare>
+  __device__ __forceinline__ void tile(const uint8_t *stage, int live, int bits, const AttnArgs &a, int64_t score_row,
+                                       int lane) {
+    const float c_hi = a.c_hi, c_lo = a.c_lo;
     const int t = lane & 3, r = lane >> 2;
+    const int offset = raw_offset<kFormat>(bits);
     float s[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
@@ -275,54 +367,73 @@ struct Worker {
       uint32_t pairs[2][S::kKeyWords * S::kPairs];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        uint32_t f = 0, rest = 0;
+        uint32_t f = 0, rest = 0, kk[S::kKeyWords];
         if constexpr (kFormat != MXQ_CACHE_BF16) {
-          f = block_factor<kFormat>(xk[h][c]) * 0x00010001u;
-          if (kBig) rest = pow2_bf16(max(xk[h][c] - 127, 0)) * 0x00010001u;
+          const uint32_t b = stage[2 * S::kSide + (r + 8 * h) * S::kScaleRow +
+                                   (((c * 4 + t) * S::kKeyPiece * 8 / S::kBits) >> 5)];
+          f = kRare ? rare_factor<kFormat>(b, offset) * 0x00010001u : b * 0x00800080u + (uint32_t)offset * 0x00800080u;
+          if (kRare) rest = rare_rest<kFormat>(b, offset) * 0x00010001u;
         }
+        load_piece<S::kKeyPiece>(stage + key_at[c & 1] + h * 8 * S::kRow + (c >> 1) * 128, kk);
 #pragma unroll
-        for (int w = 0; w < S::kKeyWords; ++w) key_word<kFormat, kBig>(kk[h][c][w], f, rest, &pairs[h][w * S::kPairs]);
+        for (int w = 0; w < S::kKeyWords; ++w) key_word<kFormat, kRare>(kk[w], f, rest, &pairs[h][w * S::kPairs]);
       }
       constexpr int kStepsHere = S::kKeyWords * S::kPairs / 2;
 #pragma unroll
       for (int k = 0; k < kStepsHere; ++k) {
-        const uint32_t a[4] = {pairs[0][2 * k], pairs[1][2 * k], pairs[0][2 * k + 1], pairs[1][2 * k + 1]};
+        const uint32_t rows[4] = {pairs[0][2 * k], pairs[1][2 * k], pairs[0][2 * k + 1], pairs[1][2 * k + 1]};
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int x = kTerms - 1; x >= 0; --x)
-            mma(s[n], a, q[x][c * kStepsHere + k][n][0], q[x][c * kStepsHere + k][n][1]);
+          for (int z = kTerms - 1; z >= 0; --z)
+            mma(s[n], rows, q[z][c * kStepsHere + k][n][0], q[z][c * kStepsHere + k][n][1]);
       }
     }
     // rows: tokens r (entries 0, 1) and r + 8 (2, 3); columns: heads 2t, 2t + 1
-    bool raise = false;
+    float x[NT][4], top = kLowest;
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[n][i] = r + 8 * (i >> 1) < live ? s[n][i] * scaling : -INFINITY;
-        raise |= s[n][i] > m[n][i & 1] + kSlack;
-      }
-    if (scores != nullptr) {
+      for (int i = 0; i < 4; ++i) x[n][i] = score(s[n][i], c_hi, c_lo, m[n][i & 1]);
+    if (live < kTile) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (r + 8 * (i >> 1) >= live) x[n][i] = -INFINITY;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, x[n][i]);
+    if (a.scores != nullptr) {
+      float *scores = a.scores + score_row * (8 * NT);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           if (r + 8 * h < live)
             *reinterpret_cast<float2 *>(scores + (int64_t)(r + 8 * h) * (8 * NT) + n * 8 + 2 * t) =
-                make_float2(s[n][2 * h], s[n][2 * h + 1]);
+                make_float2(score(s[n][2 * h], c_hi, c_lo, 0.f), score(s[n][2 * h + 1], c_hi, c_lo, 0.f));
     }
-    if (__any_sync(0xFFFFFFFFu, raise)) {
+    if (__any_sync(0xFFFFFFFFu, top > kSlack)) {
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          float top = fmaxf(s[n][h], s[n][2 + h]);
+          float y[2], high = m[n][h];
 #pragma unroll
-          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-          top = fmaxf(top, m[n][h]);
-          const float f = top == m[n][h] ? 1.f : exp2f((m[n][h] - top) * kLog2e);
-          m[n][h] = top, l[n][h] *= f;
+          for (int i = 0; i < 2; ++i) {
+            y[i] = r + 8 * i < live ? score(s[n][2 * i + h], c_hi, c_lo, 0.f) : -INFINITY;
+            high = fmaxf(high, y[i]);
+          }
+#pragma unroll
+          for (int z = 4; z < 32; z <<= 1) high = fmaxf(high, __shfl_xor_sync(0xFFFFFFFFu, high, z));
+          const float f = exp2_fast(m[n][h] - high);
+          m[n][h] = high, l[n][h] *= f;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            x[n][2 * i + h] = r + 8 * i < live ? score(s[n][2 * i + h], c_hi, c_lo, high) : -INFINITY;
 #pragma unroll
           for (int j = 0; j < kSteps; ++j) o[j][n][h] *= f, o[j][n][2 + h] *= f;
         }
@@ -333,29 +444,45 @@ struct Worker {
       float p[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        p[i] = s[n][i] == -INFINITY ? 0.f : exp2f((s[n][i] - m[n][i & 1]) * kLog2e);
+        p[i] = exp2_fast(x[n][i]);
         l[n][i & 1] += p[i];
       }
 #pragma unroll
-      for (int x = 0; x < kPTerms; ++x)
+      for (int z = 0; z < kPTerms; ++z)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          pb[x][n][h] = transpose8x8(pack_bf16x2(p[2 * h], p[2 * h + 1]));
-          p[2 * h] -= bf16_of(p[2 * h]), p[2 * h + 1] -= bf16_of(p[2 * h + 1]);
+          const uint32_t pair = pack_bf16x2(p[2 * h], p[2 * h + 1]);
+          pb[z][n][h] = transpose8x8(pair);
+          if (z + 1 < kPTerms)
+            p[2 * h] -= __uint_as_float(pair << 16), p[2 * h + 1] -= __uint_as_float(pair & 0xFFFF0000u);
         }
     }
 #pragma unroll
     for (int c = 0; c < S::kValPieces; ++c) {
-      uint32_t f[2] = {0, 0}, rest[2] = {0, 0};
+      uint32_t f[2] = {0, 0}, rest[2] = {0, 0}, vv[4][S::kValWords];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        load_piece<S::kValPiece>(stage + S::kSide + value_at[i & 1] + 8 * (i >> 1) * S::kRow + c * 128, vv[i]);
+      }
       if constexpr (kFormat != MXQ_CACHE_BF16) {
+        uint32_t b[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          b[i] = stage[2 * S::kSide + S::kScaleBytes + (2 * t + (i & 1) + 8 * (i >> 1)) * S::kScaleRow +
+                       (((c * 8 + r) * S::kValPiece * 8 / S::kBits) >> 5)];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
+          if (kRare) {
+            f[h] = rare_factor<kFormat>(b[2 * h], offset) | rare_factor<kFormat>(b[2 * h + 1], offset) << 16;
+            rest[h] = rare_rest<kFormat>(b[2 * h], offset) | rare_rest<kFormat>(b[2 * h + 1], offset) << 16;
+          } else {
+            f[h] = b[2 * h] * 128u + (b[2 * h + 1] * (128u << 16) + (uint32_t)offset * 0x00800080u);
+          }
           // a token behind the last one has factor 0: whatever its slot holds, it adds nothing
-          const uint32_t a = 2 * t + 8 * h < live ? block_factor<kFormat>(xv[2 * h][c]) : 0u;
-          const uint32_t b = 2 * t + 8 * h + 1 < live ? block_factor<kFormat>(xv[2 * h + 1][c]) : 0u;
-          f[h] = a | (b << 16);
-          if (kBig)
-            rest[h] = pow2_bf16(max(xv[2 * h][c] - 127, 0)) | (pow2_bf16(max(xv[2 * h + 1][c] - 127, 0)) << 16);
+          if (live < kTile) {
+            if (2 * t + 8 * h >= live) f[h] = 0;
+            else if (2 * t + 8 * h + 1 >= live) f[h] &= 0xFFFFu;
+          }
         }
       }
       constexpr int kPerWord = 32 / S::kBits;
@@ -364,256 +491,523 @@ struct Worker {
         uint32_t e[2][kPerWord];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          uint32_t a = vv[2 * h][c][w], b = vv[2 * h + 1][c][w];
+          uint32_t v0 = vv[2 * h][w], v1 = vv[2 * h + 1][w];
           if constexpr (kFormat == MXQ_CACHE_BF16) {
-            if (2 * t + 8 * h >= live) a = 0;
-            if (2 * t + 8 * h + 1 >= live) b = 0;
+            if (2 * t + 8 * h >= live) v0 = 0;
+            if (2 * t + 8 * h + 1 >= live) v1 = 0;
           }
-          value_words<kFormat, kBig>(a, b, f[h], rest[h], e[h]);
+          value_words<kFormat, kRare>(v0, v1, f[h], rest[h], e[h]);
         }
         constexpr int kHere = S::kValElems < kPerWord ? S::kValElems : kPerWord;
 #pragma unroll
         for (int k = 0; k < kHere; k += 2) {
           const int j = (c * S::kValElems + w * kPerWord + k) / 2;
-          const uint32_t a[4] = {e[0][k], e[0][k + 1], e[1][k], e[1][k + 1]};
+          const uint32_t rows[4] = {e[0][k], e[0][k + 1], e[1][k], e[1][k + 1]};
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
-            for (int x = kPTerms - 1; x >= 0; --x) mma(o[j][n], a, pb[x][n][0], pb[x][n][1]);
+            for (int z = kPTerms - 1; z >= 0; --z) mma(o[j][n], rows, pb[z][n][0], pb[z][n][1]);
         }
       }
     }
   }
 };
 
-// grid: (chunks, heads * head tiles, batch); the CTA's warps take the chunk's tiles in turn.
+// ---- split ---------------------------------------------------------------------------------------------------------------
+// The rows of a launch are (sequence, key/value head, head tile), each a run of units of kUnit tokens (at least one) and
+// kRowCost empty units, which stand for what beginning and ending a row costs.  The units of all rows in order are divided
+// evenly between the CTAs, whatever the lengths are: with total = q * ctas + r, CTA i takes q or (i < r) q + 1 of them.  A row inside one CTA is finished there; of a row that
+// several CTAs share each leaves an unnormalised part with its maximum and sum, and the finish kernel joins them in the
+// order of the CTAs.  A CTA shares at most its first and its last row, so there are two part slots per CTA.
+struct Split {
+  int64_t q, r;
+  __device__ __forceinline__ Split(int64_t total, int64_t ctas) {
+    if (total <= UINT32_MAX)
+      q = (uint32_t)total / (uint32_t)ctas, r = (uint32_t)total % (uint32_t)ctas;
+    else
+      q = total / ctas, r = total % ctas;
+  }
+  __device__ __forceinline__ int64_t start(int64_t i) const { return i * q + min(i, r); }
+  __device__ __forceinline__ int64_t cta_of(int64_t u) const {  // the CTA that takes unit u
+    const int64_t longer = r * (q + 1);
+    return u < longer ? u / (q + 1) : r + (u - longer) / q;
+  }
+};
+__device__ __forceinline__ int length_of(const AttnArgs &a, int b) { return clamp_length(a.lengths[b], a.most, a.status); }
+__device__ __forceinline__ int work_of_length(int n) { return max(1, (n + kUnit - 1) / kUnit); }
+__device__ __forceinline__ int units_of_length(int n) { return work_of_length(n) + kRowCost; }
+__device__ __forceinline__ int warp_sum(int v) {
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, x);
+  return v;
+}
+// units (of one row each) of the sequences first .. end - 1; called by whole warps
+__device__ __forceinline__ int64_t units_between(const AttnArgs &a, int first, int end, int lane) {
+  int64_t sum = 0;
+  for (int b0 = first; b0 < end; b0 += 32)
+    sum += warp_sum(b0 + lane < end ? units_of_length(length_of(a, b0 + lane)) : 0);
+  return sum;
+}
+// the sequence that holds unit `target` of the concatenated sequences, and the units before it
+__device__ __forceinline__ int sequence_at(const AttnArgs &a, int64_t target, int lane, int64_t &before) {
+  int64_t base = 0;
+  for (int b0 = 0;; b0 += 32) {
+    const int n = b0 + lane < a.batch ? units_of_length(length_of(a, b0 + lane)) : 0;
+    int s = n;
+#pragma unroll
+    for (int x = 1; x < 32; x <<= 1) {
+      const int y = __shfl_up_sync(0xFFFFFFFFu, s, x);
+      if (lane >= x) s += y;
+    }
+    const uint32_t past = __ballot_sync(0xFFFFFFFFu, base + s > target);
+    if (past != 0 || b0 + 32 >= a.batch) {
+      const int k = past != 0 ? __ffs(past) - 1 : 0;
+      before = base + __shfl_sync(0xFFFFFFFFu, s - n, k);
+      return min(b0 + k, a.batch - 1);
+    }
+    base += __shfl_sync(0xFFFFFFFFu, s, 31);
+  }
+}
+
+// Place of a unit in the rows.
+struct Cursor {
+  int b, row, unit, units, length;
+  // to the next unit; `more`: there is one
+  __device__ __forceinline__ void advance(const AttnArgs &a, int rows, bool more) {
+    if (++unit < units) return;
+    unit = 0;
+    if (++row < rows) return;
+    row = 0;
+    if (more) length = length_of(a, ++b), units = units_of_length(length);
+  }
+};
+
+template <int kFormat, int D, int NT>
+struct Smem {
+  static constexpr int kRing = kWarps * Shape<kFormat, D>::kStages * Shape<kFormat, D>::kStage;
+  static constexpr int kJoin = kWarps * 8 * NT * (D + 2) * 4;
+  static constexpr int kTotal = kRing + kJoin;
+};
+
+// Any of the four scale bytes outside of the plain range of factors?
+template <int kFormat>
+__device__ __forceinline__ bool any_rare(uint32_t w, int bits) {
+  const uint32_t low = w & 0x7F7F7F7Fu;
+  if constexpr (kFormat == MXQ_CACHE_INT8) {
+    const uint32_t small = ~((low + (uint32_t)(128 - bits) * 0x01010101u) | w);  // byte < bits
+    return ((small | ((low + 0x01010101u) & w)) & 0x80808080u) != 0;             // or byte == 255
+  } else {
+    const uint32_t limit = 254 - raw_offset<kFormat>(0);  // 128 .. 142: rare above it
+    return ((low + (255u - limit) * 0x01010101u) & w & 0x80808080u) != 0;
+  }
+}
+
 template <typename T, int kFormat, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32)
+__global__ void __launch_bounds__(kWarps * 32, Elem<T>::kBf16 && D == 128 && NT == 1 ? 4 : 1)
 attention_kernel(const Cache c, const Table table, const AttnArgs a) {
   using S = Shape<kFormat, D>;
-  __shared__ float sm_o[kWarps][NT * 8][D];
-  __shared__ float sm_m[kWarps][NT * 8], sm_l[kWarps][NT * 8];
+  constexpr int kHeads = 8 * NT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  float *sm_o = reinterpret_cast<float *>(smem + Smem<kFormat, D, NT>::kRing);  // [kWarps][kHeads * D / 32][32]
+  float *sm_m = sm_o + kWarps * kHeads * D, *sm_l = sm_m + kWarps * kHeads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int t = lane & 3, r = lane >> 2;
-  const int head = blockIdx.y / a.head_tiles, ht = blockIdx.y - head * a.head_tiles;
-  const int64_t b = blockIdx.z;
-  const int length = clamp_length(a.lengths[b], a.most, a.status);
-  const int begin = blockIdx.x * a.chunk, end = min(begin + a.chunk, length);
-  if (begin >= end && !(blockIdx.x == 0 && a.chunks == 1)) return;
-  const int first_head = head * a.group + ht * (8 * NT);
-  const int heads = min(a.group - ht * (8 * NT), 8 * NT);
+  uint8_t *ring = smem + warp * (S::kStages * S::kStage);
 
+  const int rows = c.heads * a.head_tiles;
+  const int64_t total = units_between(a, 0, a.batch, lane) * rows;
+  const int64_t ctas = min((int64_t)a.ctas, total);
+  if (blockIdx.x >= ctas) return;
+  const Split split(total, ctas);
+  const int64_t begin = split.start(blockIdx.x);
+  const int todo = (int)(split.start(blockIdx.x + 1) - begin);  // the host bounds the units of a launch
+  Cursor here;  // the unit being worked on
+  {
+    int64_t before;
+    const int64_t target = total <= UINT32_MAX ? (uint32_t)begin / (uint32_t)rows : begin / rows;
+    here.b = sequence_at(a, target, lane, before);
+    here.length = length_of(a, here.b), here.units = units_of_length(here.length);
+    const int64_t in_seq = begin - before * rows;
+    here.row = (int)(in_seq <= UINT32_MAX ? (uint32_t)in_seq / (uint32_t)here.units : in_seq / here.units);
+    here.unit = (int)(in_seq - (int64_t)here.row * here.units);
+  }
+
+  // Where the warp's tiles lie is worked out for 32 units at a time, one per lane: `place` is the byte offset of the
+  // lane's tile (of the batch of units in use) from the start of the pages, `entry` and `entry_off` are the page table
+  // entry and the offset inside the page for the batch after it, whose loads have 32 units of time to arrive.
+  Cursor ahead = here;  // first unit of the batch that is looked up next
+  int looked_up = 0;    // units looked up
+  int entry = 0;
+  uint32_t entry_off = 0;
+  uint64_t place = 0;
+  constexpr uint32_t kNoTile = 0xFFFFFFFFu;
+  constexpr uint64_t kNoPlace = ~0ull;
+  const uint32_t page_bytes = (uint32_t)(c.heads << c.page_log2) * S::kRow;  // below 2^32: at most 32767 heads
+  auto look_up = [&]() {
+    Cursor mine = ahead;
+    int64_t pos = (int64_t)mine.row * mine.units + mine.unit + lane;  // place in the units of all rows of the sequence
+    const bool any = looked_up + lane < todo;
+    while (any && pos >= (int64_t)rows * mine.units) {
+      pos -= (int64_t)rows * mine.units;
+      mine.length = length_of(a, ++mine.b), mine.units = units_of_length(mine.length);
+    }
+    if (any) {
+      mine.row = (int)(pos <= UINT32_MAX ? (uint32_t)pos / (uint32_t)mine.units : pos / mine.units);
+      mine.unit = (int)(pos - (int64_t)mine.row * mine.units);
+    }
+    const int tok = mine.unit * kUnit + warp * kTile;
+    entry_off = kNoTile;
+    if (any && tok < mine.length) {
+      entry = table.entries[mine.b * table.stride + (tok >> c.page_log2)];
+      const int head = a.head_tiles == 1 ? mine.row : mine.row / a.head_tiles;
+      entry_off = (uint32_t)((head << c.page_log2) + (tok & ((1 << c.page_log2) - 1))) * S::kRow;
+    }
+    looked_up += 32;
+    if (looked_up < todo) {  // every lane had a unit: go on behind the last one
+      ahead.b = __shfl_sync(0xFFFFFFFFu, mine.b, 31), ahead.row = __shfl_sync(0xFFFFFFFFu, mine.row, 31);
+      ahead.unit = __shfl_sync(0xFFFFFFFFu, mine.unit, 31), ahead.units = __shfl_sync(0xFFFFFFFFu, mine.units, 31);
+      ahead.length = __shfl_sync(0xFFFFFFFFu, mine.length, 31);
+      ahead.advance(a, rows, true);
+    }
+  };
+  auto settle = [&]() {
+    place = kNoPlace;
+    if (entry_off != kNoTile) {
+      if (entry < 0 || entry >= c.pages)
+        report(a.status);
+      else
+        place = (uint64_t)(uint32_t)entry * page_bytes + entry_off;
+    }
+  };
+  const int key_to = S::key_slot(lane * 16 / S::kRow, lane * 16 % S::kRow);
+  const int value_to = S::value_slot(lane * 16 / S::kRow, lane * 16 % S::kRow);
+  uint32_t absent = 0;  // bit s: the tile in stage s does not exist
+  auto issue = [&](int unit, int stage) {  // copies the warp's tile of a unit of the batch in use
+    const uint64_t off = __shfl_sync(0xFFFFFFFFu, place, unit & 31);
+    if (off != kNoPlace) {
+      absent &= ~(1u << stage);
+      uint8_t *dst = ring + stage * S::kStage;
+      const uint8_t *kp = c.codes[0] + off + lane * 16, *vp = c.codes[1] + off + lane * 16;
+#pragma unroll
+      for (int i = 0; i < S::kSide; i += 512)
+        if (S::kSide % 512 == 0 || lane * 16 < S::kSide) {
+          copy_async<16>(dst + i + (key_to ^ S::key_turn(i)), kp + i);
+          copy_async<16>(dst + S::kSide + i + (value_to ^ S::value_turn(i)), vp + i);
+        }
+      if constexpr (kFormat != MXQ_CACHE_BF16) {
+        constexpr int kPerScale = S::kRow / S::kScaleRow;  // code bytes of a block: 32 or 16
+#pragma unroll
+        for (int i = 0; i < 8 * S::kScaleRow; i += 32) {
+          const int word = i + lane, side = word >= 4 * S::kScaleRow;
+          if (8 * S::kScaleRow % 32 == 0 || word < 8 * S::kScaleRow)
+            copy_async<4>(dst + 2 * S::kSide + word * 4,
+                          (side ? c.scales[1] : c.scales[0]) + (word - side * 4 * S::kScaleRow) * 4 + off / kPerScale);
+        }
+      }
+    } else {
+      absent |= 1u << stage;
+    }
+    copy_commit();
+  };
+
+  look_up();
+  settle();
+  if (looked_up < todo) look_up();
+#pragma unroll
+  for (int k = 0; k < S::kStages - 1; ++k) {
+    if (k < todo)
+      issue(k, k);
+    else
+      copy_commit();
+  }
+
+  auto tile_of_head = [&](const Cursor &at, int &first_head, int &heads) {
+    const int head = a.head_tiles == 1 ? at.row : at.row / a.head_tiles, ht = at.row - head * a.head_tiles;
+    first_head = head * a.group + ht * kHeads, heads = min(a.group - ht * kHeads, kHeads);
+  };
   Worker<T, kFormat, D, NT> w;
-  w.start(static_cast<const T *>(a.q) + b * a.q_stride_b + first_head * a.q_stride_h, a.q_stride_h, heads, lane);
-  float *scores = a.scores == nullptr
-                      ? nullptr
-                      : a.scores + (((b * c.heads + head) * a.head_tiles + ht) * a.score_tokens) * (8 * NT);
-  const int in_page = (1 << c.page_log2) - 1;
-  for (int tok = begin + warp * kTile; tok < end; tok += kWarps * kTile) {
-    const int live = end - tok;
-    const int64_t first = page_row(c, table, b, head, tok, a.status);
-    if (first < 0) {  // the page does not exist: its tokens are left out
-      if (scores != nullptr)
-        for (int i = lane; i < min(live, kTile) * 8 * NT; i += 32) scores[(int64_t)tok * (8 * NT) + i] = -INFINITY;
+  int first_head, heads;
+  auto load_query = [&](const Cursor &at, int first, int n) {
+    w.load_query(static_cast<const T *>(a.q) + at.b * a.q_stride_b + first * a.q_stride_h, a.q_stride_h, n, lane);
+  };
+  w.setup(lane);
+  w.clear();
+  tile_of_head(here, first_head, heads);
+  load_query(here, first_head, heads);
+  int from = 0, from_unit = here.unit;  // where the CTA's part of the row begins: in its own units, in the row's
+  bool joined = false;
+  for (int i = 0, stage = 0; i < todo; ++i) {
+    copy_wait<S::kStages - 2>();
+    __syncwarp();  // the scale bytes were copied by other lanes; and all lanes are done with the stage before this one
+    const int fill = i + S::kStages - 1;
+    if (fill < todo) {
+      if ((fill & 31) == 0) {
+        settle();
+        if (looked_up < todo) look_up();
+      }
+      issue(fill, stage == 0 ? S::kStages - 1 : stage - 1);
+    } else {
+      copy_commit();
+    }
+    const int work = here.units - kRowCost;
+    const int tok = here.unit * kUnit + warp * kTile;
+    const int live = here.length - tok;
+    if ((absent >> stage) & 1u) {  // behind the end, or the page does not exist: its tokens are left out
+      if (a.scores != nullptr) {
+        float *sc = a.scores + (((int64_t)here.b * rows + here.row) * a.score_tokens + tok) * kHeads;
+        for (int j = lane; j < min(live, kTile) * kHeads; j += 32) sc[j] = -INFINITY;
+      }
+    } else {
+      const uint8_t *st = ring + stage * S::kStage;
+      bool rare = false;
+      if constexpr (kFormat != MXQ_CACHE_BF16) {
+#pragma unroll
+        for (int j = 0; j < 8 * S::kScaleRow; j += 32)
+          if (8 * S::kScaleRow % 32 == 0 || j + lane < 8 * S::kScaleRow)
+            rare |= any_rare<kFormat>(reinterpret_cast<const uint32_t *>(st + 2 * S::kSide)[j + lane], c.bits);
+        rare = __any_sync(0xFFFFFFFFu, rare);
+      }
+      if (kFormat != MXQ_CACHE_BF16 && rare)
+        w.template tile<true>(st, live, c.bits, a, ((int64_t)here.b * rows + here.row) * a.score_tokens + tok, lane);
+      else
+        w.template tile<false>(st, live, c.bits, a, ((int64_t)here.b * rows + here.row) * a.score_tokens + tok, lane);
+    }
+    stage = stage == S::kStages - 1 ? 0 : stage + 1;
+    if (i + 1 == todo) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (here.unit + 1 < work && i + 1 < todo) {
+      ++here.unit;
       continue;
     }
-    const int64_t row = first + (tok & in_page);
-    uint32_t kk[2][S::kKeyPieces][S::kKeyWords], vv[4][S::kValPieces][S::kValWords];
-    int xk[2][S::kKeyPieces], xv[4][S::kValPieces];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint8_t *p = c.codes[0] + (row + r + 8 * h) * S::kRow + t * S::kKeyPiece;
-#pragma unroll
-      for (int k = 0; k < S::kKeyPieces; ++k) load_piece<S::kKeyPiece>(p + k * 4 * S::kKeyPiece, kk[h][k]);
+    const bool ends = here.unit < work;  // the CTA's part of the row ends here (otherwise an empty unit)
+    const int slot = from > 0, b_now = here.b, head_now = first_head, heads_now = heads;
+    const bool whole = from_unit == 0 && here.unit + 1 == work;
+    here.advance(a, rows, i + 1 < todo);
+    if (here.unit == 0) {  // the next row's queries are on their way while this row is joined
+      from = i + 1, from_unit = 0;
+      if (i + 1 < todo) tile_of_head(here, first_head, heads), load_query(here, first_head, heads);
     }
+    if (!ends) continue;
+
+    // Join the warps.  Every lane holds heads 2t, 2t + 1 of each tile (entry & 1) at two rows of O^T (entry >> 1) for each
+    // of D / 16 steps; sums run over the lanes of equal t.
+    if (joined) __syncthreads();  // the previous join has been read
+    joined = true;
+    constexpr int kEntries = NT * D / 4;  // of a lane: [n][h][2 j + row]
+    float *mine = sm_o + warp * kEntries * 32 + lane;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint8_t *p = c.codes[1] + (row + 2 * t + (i & 1) + 8 * (i >> 1)) * S::kRow + r * S::kValPiece;
-#pragma unroll
-      for (int k = 0; k < S::kValPieces; ++k) load_piece<S::kValPiece>(p + k * 8 * S::kValPiece, vv[i][k]);
-    }
-    bool big = false;
-    if constexpr (kFormat != MXQ_CACHE_BF16) {
+    for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const uint8_t *p = c.scales[0] + (row + r + 8 * h) * (D / 32);
+        float l = w.l[n][h];
 #pragma unroll
-        for (int k = 0; k < S::kKeyPieces; ++k)
-          xk[h][k] = block_exponent<kFormat>(p[((k * 4 + t) * S::kKeyPiece * 8 / S::kBits) >> 5], c.bits);
-      }
+        for (int y = 4; y < 32; y <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, y);
+        const int hh = warp * kHeads + n * 8 + 2 * t + h;
+        if (r == 0) sm_m[hh] = w.m[n][h], sm_l[hh] = l;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint8_t *p = c.scales[1] + (row + 2 * t + (i & 1) + 8 * (i >> 1)) * (D / 32);
-#pragma unroll
-        for (int k = 0; k < S::kValPieces; ++k)
-          xv[i][k] = block_exponent<kFormat>(p[((k * 8 + r) * S::kValPiece * 8 / S::kBits) >> 5], c.bits);
-      }
-      if constexpr (kFormat != MXQ_CACHE_INT8) {
-#pragma unroll
-        for (int k = 0; k < S::kKeyPieces; ++k) big |= xk[0][k] > 127 || xk[1][k] > 127;
-#pragma unroll
-        for (int k = 0; k < S::kValPieces; ++k)
-          big |= xv[0][k] > 127 || xv[1][k] > 127 || xv[2][k] > 127 || xv[3][k] > 127;
-        big = __any_sync(0xFFFFFFFFu, big);
+        for (int e = 0; e < D / 8; ++e) mine[((n * 2 + h) * (D / 8) + e) * 32] = w.o[e >> 1][n][2 * (e & 1) + h];
       }
     }
-    float *sc = scores == nullptr ? nullptr : scores + (int64_t)tok * (8 * NT);
-    if (kFormat != MXQ_CACHE_BF16 && kFormat != MXQ_CACHE_INT8 && big)
-      w.template tile<true>(kk, vv, xk, xv, live, a.scaling, sc, lane);
-    else
-      w.template tile<false>(kk, vv, xk, xv, live, a.scaling, sc, lane);
-  }
-
-  // join the warps: every lane holds heads 2t, 2t + 1 of each tile; sums run over the lanes of equal t
+    w.clear();
+    __syncthreads();
+    // a warp takes a quarter of the entries of its lanes' heads: 8 or fewer neighbouring elements of a head
+    constexpr int kQuarter = kEntries / kWarps;
+    const int e0 = warp * kQuarter, h = (e0 / (D / 8) / 2) * 8 + 2 * t + ((e0 / (D / 8)) & 1);
+    if (h < heads_now) {
+      float top = sm_m[h], f[kWarps], sum = 0.f;
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
+      for (int k = 1; k < kWarps; ++k) top = fmaxf(top, sm_m[k * kHeads + h]);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      float l = w.l[n][h];
+      for (int k = 0; k < kWarps; ++k) f[k] = exp2f(sm_m[k * kHeads + h] - top), sum += f[k] * sm_l[k * kHeads + h];
+      const int64_t head_row = (int64_t)b_now * a.q_heads + head_now + h;
+      const int64_t part = ((int64_t)blockIdx.x * 2 + slot) * kHeads + h;
 #pragma unroll
-      for (int x = 4; x < 32; x <<= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
-      if (r == 0) sm_m[warp][n * 8 + 2 * t + h] = w.m[n][h], sm_l[warp][n * 8 + 2 * t + h] = l;
+      for (int e = 0; e < kQuarter; ++e) {
+        float v = 0.f;
 #pragma unroll
-      for (int j = 0; j < D / 16; ++j) {
-        sm_o[warp][n * 8 + 2 * t + h][value_element<kFormat, D>(2 * j, r)] = w.o[j][n][h];
-        sm_o[warp][n * 8 + 2 * t + h][value_element<kFormat, D>(2 * j + 1, r)] = w.o[j][n][2 + h];
+        for (int k = 0; k < kWarps; ++k) v += f[k] * sm_o[(k * kEntries + e0 + e) * 32 + lane];
+        const int d = value_element<kFormat, D>((e0 + e) % (D / 8), r);
+        if (whole)
+          store_scalar(static_cast<T *>(a.out) + head_row * D + d, sum == 0.f ? 0.f : v / sum);
+        else
+          a.part_o[part * D + d] = v;
       }
-    }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < heads * D; i += kWarps * 32) {
-    const int h = i / D, d = i - h * D;
-    float top = sm_m[0][h];
-#pragma unroll
-    for (int k = 1; k < kWarps; ++k) top = fmaxf(top, sm_m[k][h]);
-    float sum = 0.f, v = 0.f;
-#pragma unroll
-    for (int k = 0; k < kWarps; ++k) {
-      const float f = sm_m[k][h] == -INFINITY ? 0.f : exp2f((sm_m[k][h] - top) * kLog2e);
-      sum += f * sm_l[k][h], v += f * sm_o[k][h][d];
-    }
-    const int64_t head_row = b * a.q_heads + first_head + h;
-    if (a.part_o == nullptr) {
-      store_scalar(static_cast<T *>(a.out) + head_row * D + d, sum > 0.f ? v / sum : (sum == 0.f ? 0.f : sum));
-    } else {
-      const int64_t part = head_row * a.chunks + blockIdx.x;
-      a.part_o[part * D + d] = v;
-      if (d == 0) a.part_ml[part] = make_float2(top, sum);
+      if (r == 0 && e0 % (D / 8) == 0) {
+        if (!whole)
+          a.part_ml[part] = make_float2(top, sum);
+        else if (a.stats != nullptr)
+          a.stats[head_row] = make_float2(top, sum);
+      }
     }
   }
 }
 
-// Maximum and sum over a head's chunks; every thread of a warp gets them.
-__device__ __forceinline__ float2 join_stats(const float2 *ml, int n, int lane) {
-  float top = -INFINITY;
-  for (int k = lane; k < n; k += 32) top = fmaxf(top, ml[k].x);
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-  float sum = 0.f;
-  for (int k = lane; k < n; k += 32) sum += ml[k].x == -INFINITY ? ml[k].y : ml[k].y * exp2f((ml[k].x - top) * kLog2e);
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
-  return make_float2(top, sum);
-}
-
-// grid: (query heads, batch); threads over head_dim
+// Joins the parts of the rows that CTAs share, and adds the softmax weights of every token to the caller's statistics:
+//   weights[b, head, j] += sum over the group of exp(s_j - m) / l.
+// grid: (x, heads, batch): heads g of a group with g % x == blockIdx.x are joined by the CTA, tokens are strided over x.
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttnArgs a, int dim) {
-  const int head = blockIdx.x;
-  const int64_t b = blockIdx.y, row = b * a.q_heads + head;
-  const int length = clamp_length(a.lengths[b], a.most, a.status);
-  const int n = (length + a.chunk - 1) / a.chunk;
-  const float2 *ml = a.part_ml + row * a.chunks;
-  const float2 st = join_stats(ml, n, threadIdx.x & 31);
-  for (int d = threadIdx.x; d < dim; d += kJoinThreads) {
-    float v = 0.f;
-    for (int k = 0; k < n; ++k) {
-      const float f = ml[k].x == -INFINITY ? 0.f : exp2f((ml[k].x - st.x) * kLog2e);
-      v += f * a.part_o[(row * a.chunks + k) * dim + d];
-    }
-    store_scalar(static_cast<T *>(a.out) + row * dim + d, st.y > 0.f ? v / st.y : (st.y == 0.f ? 0.f : st.y));
-  }
-}
+__global__ void __launch_bounds__(kFinishThreads)
+finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
+  extern __shared__ float sm[];  // [4][dim] sums of the warps, then [group] pairs of maximum and 1 / sum
+  float2 *stats = reinterpret_cast<float2 *>(sm + 4 * dim);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int head = blockIdx.y, b = blockIdx.z;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int rows = heads * a.head_tiles;
+  const int64_t before = units_between(a, 0, b, lane);
+  const int n = units_of_length(length_of(a, b));
+  const int64_t total = (before + units_between(a, b, a.batch, lane)) * rows;
+  const Split split(total, min((int64_t)a.ctas, total));
 
-// weights[b, head, j] += sum over the group of exp(s_j - m) / l.  grid: (token chunks, heads, batch)
-__global__ void __launch_bounds__(kJoinThreads) weights_kernel(const AttnArgs a, int heads, int tile_heads) {
-  extern __shared__ float2 stats[];  // [group]: maximum, 1 / sum
-  const int head = blockIdx.y, lane = threadIdx.x & 31;
-  const int64_t b = blockIdx.z;
-  const int length = clamp_length(a.lengths[b], a.most, a.status);
-  const int n = (length + a.chunk - 1) / a.chunk;
-  for (int g = threadIdx.x >> 5; g < a.group; g += kJoinThreads / 32) {
-    const float2 st = join_stats(a.part_ml + (b * a.q_heads + head * a.group + g) * a.chunks, n, lane);
+  // CTAs first .. last hold the parts of head g's row; part of CTA c in its slot 0 or 1
+  auto locate = [&](int g, int64_t &first, int64_t &last, bool &late) {
+    const int64_t u0 = before * rows + (int64_t)(head * a.head_tiles + g / tile_heads) * n;
+    first = split.cta_of(u0), last = split.cta_of(u0 + n - kRowCost - 1);
+    late = split.start(first) < u0;  // the row is not the first one of its first CTA
+  };
+  auto part_of = [&](int64_t c, int64_t first, bool late, int g) {
+    return (c * 2 + (c == first && late ? 1 : 0)) * tile_heads + g % tile_heads;
+  };
+  // maximum and sum of head g, by a whole warp
+  auto join = [&](int g) {
+    int64_t first, last;
+    bool late;
+    locate(g, first, last, late);
+    if (first == last) return a.stats != nullptr ? a.stats[(int64_t)b * a.q_heads + head * a.group + g] : make_float2(0.f, 0.f);
+    float top = kLowest;
+    for (int64_t c = first + lane; c <= last; c += 32) top = fmaxf(top, a.part_ml[part_of(c, first, late, g)].x);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
+    float sum = 0.f;
+    for (int64_t c = first + lane; c <= last; c += 32) {
+      const float2 p = a.part_ml[part_of(c, first, late, g)];
+      sum += p.y * exp2f(p.x - top);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+    return make_float2(top, sum);
+  };
+
+  for (int g = blockIdx.x; g < a.group; g += gridDim.x) {
+    int64_t first, last;
+    bool late;
+    locate(g, first, last, late);
+    if (first == last) continue;  // finished by its CTA
+    const float2 st = join(g);
+    for (int d0 = 0; d0 < dim; d0 += 32) {
+      float v = 0.f;
+      for (int64_t c = first + warp; c <= last; c += 4) {
+        const int64_t part = part_of(c, first, late, g);
+        v += exp2f(a.part_ml[part].x - st.x) * a.part_o[part * dim + d0 + lane];
+      }
+      sm[warp * dim + d0 + lane] = v;
+    }
+    __syncthreads();
+    for (int d = threadIdx.x; d < dim; d += kFinishThreads) {
+      const float v = sm[d] + sm[dim + d] + sm[2 * dim + d] + sm[3 * dim + d];
+      store_scalar(static_cast<T *>(a.out) + ((int64_t)b * a.q_heads + head * a.group + g) * dim + d,
+                   st.y == 0.f ? 0.f : v / st.y);
+    }
+    __syncthreads();
+  }
+  if (a.weights == nullptr) return;
+  for (int g = warp; g < a.group; g += kFinishThreads / 32) {
+    const float2 st = join(g);
     if (lane == 0) stats[g] = make_float2(st.x, st.y == 0.f ? 0.f : 1.f / st.y);
   }
   __syncthreads();
-  for (int j = blockIdx.x * kJoinThreads + threadIdx.x; j < length; j += gridDim.x * kJoinThreads) {
+  const int length = length_of(a, b);
+  for (int j = blockIdx.x * kFinishThreads + threadIdx.x; j < length; j += gridDim.x * kFinishThreads) {
     float sum = 0.f;
     for (int g = 0; g < a.group; ++g) {
-      const int ht = g / tile_heads;
-      const float s = a.scores[(((b * heads + head) * a.head_tiles + ht) * a.score_tokens + j) * tile_heads + g % tile_heads];
-      sum += s == -INFINITY ? 0.f : exp2f((s - stats[g].x) * kLog2e) * stats[g].y;
+      const int64_t row = (int64_t)b * rows + head * a.head_tiles + g / tile_heads;
+      const float s = a.scores[(row * a.score_tokens + j) * tile_heads + g % tile_heads];
+      sum += exp2f(s - stats[g].x) * stats[g].y;
     }
-    a.weights[(b * heads + head) * a.weights_width + j] += sum;
+    a.weights[((int64_t)b * heads + head) * a.weights_width + j] += sum;
   }
 }
 
-// How a call is split: query heads in tiles of 8 (16 for bf16 queries of more than 8 heads a group and head_dim <= 128),
-// the length in chunks so that the launch has about two CTAs' worth of work for each of the four a SM holds.
-struct Plan {
-  int nt, head_tiles, chunk, chunks;
-};
-static Plan plan_of(int dtype, int dim, int64_t group, int64_t heads, int64_t batch, int64_t tokens) {
-  Plan p;
-  p.nt = dtype == MXQ_BF16 && group > 8 && dim <= 128 ? 2 : 1;
-  p.head_tiles = (int)((group + 8 * p.nt - 1) / (8 * p.nt));
-  const int64_t rows = heads * p.head_tiles * batch;
-  int64_t chunk = (tokens * rows + gemm::sm_count() * 8 - 1) / (gemm::sm_count() * 8);
-  chunk = (chunk + 63) / 64 * 64;
-  if (chunk < 64) chunk = 64;
-  p.chunk = (int)chunk;
-  p.chunks = (int)((tokens + chunk - 1) / chunk);
-  return p;
+// Query heads in tiles of 8, or of 16 for bf16 queries of more than 8 heads a group and head_dim <= 128 (larger ones do
+// not fit the registers).
+static int tiles_per_row(int dtype, int dim, int64_t group) { return dtype == MXQ_BF16 && group > 8 && dim <= 128 ? 2 : 1; }
+constexpr int kMostPerSm = 8;  // CTAs of the attention kernel on one SM, at most
+
+static int64_t units_of_launch(int64_t batch, int64_t rows, int64_t tokens) {
+  return batch * rows * ((tokens + kUnit - 1) / kUnit + kRowCost);
 }
 struct Workspace {
-  int64_t ml, o, scores, total;  // byte offsets
+  int64_t ml, o, stats, scores, total;  // byte offsets
 };
-static Workspace workspace_of(const Plan &p, int64_t batch, int64_t heads, int64_t q_heads, int dim, int64_t tokens,
-                              bool weights) {
-  Workspace w;
+static Workspace workspace_of(int nt, int64_t batch, int64_t heads, int64_t q_heads, int dim, int64_t tokens, bool weights,
+                              int64_t &most_ctas) {
+  const int64_t head_tiles = (q_heads / heads + 8 * nt - 1) / (8 * nt);
+  const int64_t units = units_of_launch(batch, heads * head_tiles, tokens);
+  most_ctas = (int64_t)gemm::sm_count() * kMostPerSm;
+  if (units < most_ctas) most_ctas = units;
   auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
-  const bool parts = p.chunks > 1 || weights;
+  const bool parts = tokens > kUnit;
+  Workspace w;
   w.ml = 0;
-  w.o = parts ? up(batch * q_heads * p.chunks * (int64_t)sizeof(float2)) : 0;
-  w.scores = w.o + (parts ? up(batch * q_heads * p.chunks * (int64_t)dim * 4) : 0);
-  w.total = w.scores + (weights ? batch * heads * p.head_tiles * tokens * (8 * p.nt) * 4 : 0);
+  w.o = parts ? up(most_ctas * 2 * 8 * nt * (int64_t)sizeof(float2)) : 0;
+  w.stats = w.o + (parts ? up(most_ctas * 2 * 8 * nt * dim * 4) : 0);
+  w.scores = w.stats + (weights ? up(batch * q_heads * (int64_t)sizeof(float2)) : 0);
+  w.total = w.scores + (weights ? batch * heads * head_tiles * tokens * (8 * nt) * 4 : 0);
   return w;
 }
 
-template <typename T, int kFormat, int D>
-static void launch_attention(const Cache &c, const Table &t, const AttnArgs &a, const Plan &p, int64_t batch,
-                             cudaStream_t st) {
-  const dim3 grid((unsigned)p.chunks, (unsigned)(c.heads * p.head_tiles), (unsigned)batch);
-  if constexpr (Elem<T>::kBf16 && D <= 128) {
-    if (p.nt == 2) {
-      attention_kernel<T, kFormat, D, 2><<<grid, kWarps * 32, 0, st>>>(c, t, a);
-      return;
-    }
+template <typename T, int kFormat, int D, int NT>
+static int launch_one(const Cache &c, const Table &t, AttnArgs &a, int64_t most_ctas, cudaStream_t st) {
+  constexpr int kSmem = Smem<kFormat, D, NT>::kTotal;
+  auto kernel = attention_kernel<T, kFormat, D, NT>;
+  int per_sm = 0;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kWarps * 32, kSmem) != cudaSuccess || per_sm < 1) {
+    cudaGetLastError();
+    return MXQ_ERR_LAUNCH;
   }
-  attention_kernel<T, kFormat, D, 1><<<grid, kWarps * 32, 0, st>>>(c, t, a);
+  int64_t ctas = (int64_t)gemm::sm_count() * (per_sm < kMostPerSm ? per_sm : kMostPerSm);
+  if (ctas > most_ctas) ctas = most_ctas;
+  a.ctas = (int)ctas;
+  kernel<<<(unsigned)ctas, kWarps * 32, kSmem, st>>>(c, t, a);
+  return cudaGetLastError() == cudaSuccess ? MXQ_OK : MXQ_ERR_LAUNCH;
+}
+template <typename T, int kFormat, int D>
+static int launch_dim(const Cache &c, const Table &t, AttnArgs &a, int nt, int64_t most_ctas, cudaStream_t st) {
+  if constexpr (Elem<T>::kBf16 && D <= 128) {
+    if (nt == 2) return launch_one<T, kFormat, D, 2>(c, t, a, most_ctas, st);
+  }
+  return launch_one<T, kFormat, D, 1>(c, t, a, most_ctas, st);
 }
 template <typename T>
-static void launch_attention(int format, int dim, const Cache &c, const Table &t, const AttnArgs &a, const Plan &p,
-                             int64_t batch, cudaStream_t st) {
-#define CALL(f)                                                              \
-  if (format == f) {                                                         \
-    if (dim == 32) launch_attention<T, f, 32>(c, t, a, p, batch, st);        \
-    if (dim == 64) launch_attention<T, f, 64>(c, t, a, p, batch, st);        \
-    if (dim == 128) launch_attention<T, f, 128>(c, t, a, p, batch, st);      \
-    if (dim == 256) launch_attention<T, f, 256>(c, t, a, p, batch, st);      \
+static int launch_attention(int format, int dim, const Cache &c, const Table &t, AttnArgs &a, int nt, int64_t most_ctas,
+                            cudaStream_t st) {
+#define CALL(f)                                                                      \
+  if (format == f) {                                                                 \
+    if (dim == 32) return launch_dim<T, f, 32>(c, t, a, nt, most_ctas, st);          \
+    if (dim == 64) return launch_dim<T, f, 64>(c, t, a, nt, most_ctas, st);          \
+    if (dim == 128) return launch_dim<T, f, 128>(c, t, a, nt, most_ctas, st);        \
+    if (dim == 256) return launch_dim<T, f, 256>(c, t, a, nt, most_ctas, st);        \
   }
   MXQ_PAGED_FORMATS(CALL)
 #undef CALL
+  return MXQ_ERR_FORMAT;
+}
+
+// The finish kernel is launched while the attention kernel drains and waits on the device for its end.
+template <typename T>
+static int launch_finish(const AttnArgs &a, int heads, int tile_heads, int dim, unsigned x, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(x, (unsigned)heads, (unsigned)a.batch), cfg.blockDim = dim3(kFinishThreads);
+  cfg.dynamicSmemBytes = 4 * dim * 4 + (a.weights != nullptr ? a.group * sizeof(float2) : 0), cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr, cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, finish_kernel<T>, a, heads, tile_heads, dim) != cudaSuccess) {
+    cudaGetLastError();
+    return MXQ_ERR_LAUNCH;
+  }
+  return MXQ_OK;
 }
 
 }  // namespace paged
@@ -644,8 +1038,9 @@ int64_t mxq_paged_attention_workspace_bytes(const mxq_paged_cache *cache, int64_
   const int64_t tokens = table_width << c.page_log2;
   int64_t most = 0;
   for (int dtype : {MXQ_F32, MXQ_BF16}) {
-    const Plan p = plan_of(dtype, cache->head_dim, group, c.heads, batch, tokens);
-    const int64_t n = workspace_of(p, batch, c.heads, q_heads, cache->head_dim, tokens, with_weights != 0).total;
+    int64_t ctas;
+    const int nt = tiles_per_row(dtype, cache->head_dim, group);
+    const int64_t n = workspace_of(nt, batch, c.heads, q_heads, cache->head_dim, tokens, with_weights != 0, ctas).total;
     if (n > most) most = n;
   }
   return most;
@@ -667,9 +1062,12 @@ int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, 
   if (weights && weights_width < 1) return MXQ_ERR_SHAPE;
   const int dim = cache->head_dim;
   const int64_t tokens = table_width << c.page_log2;
-  const Plan p = plan_of(dtype, dim, group, c.heads, batch, tokens);
-  if ((int64_t)c.heads * p.head_tiles > 65535) return MXQ_ERR_SHAPE;
-  const Workspace w = workspace_of(p, batch, c.heads, q_heads, dim, tokens, weights != nullptr);
+  const int nt = tiles_per_row(dtype, dim, group);
+  int64_t most_ctas;
+  const Workspace w = workspace_of(nt, batch, c.heads, q_heads, dim, tokens, weights != nullptr, most_ctas);
+  // a CTA counts its units in 32 bits: with one CTA on each SM it has at most this many
+  if (units_of_launch(batch, c.heads * ((group + 8 * nt - 1) / (8 * nt)), tokens) / gemm::sm_count() >= INT32_MAX)
+    return MXQ_ERR_SHAPE;
   if (w.total > 0) {
     if (!workspace) return MXQ_ERR_NULL;
     if (!aligned(workspace, 16)) return MXQ_ERR_ALIGN;
@@ -677,40 +1075,32 @@ int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, 
   }
   uint8_t *ws = static_cast<uint8_t *>(workspace);
   AttnArgs a;
-  a.q = q, a.out = out, a.q_stride_b = q_stride_b, a.q_stride_h = q_stride_h, a.scaling = scaling;
-  a.group = (int)group, a.q_heads = (int)q_heads, a.head_tiles = p.head_tiles;
-  a.lengths = lengths;
+  a.q = q, a.out = out, a.q_stride_b = q_stride_b, a.q_stride_h = q_stride_h;
+  const double factor = (double)scaling * 1.4426950408889634074;
+  a.c_hi = (float)factor, a.c_lo = (float)(factor - a.c_hi);
+  a.group = (int)group, a.q_heads = (int)q_heads, a.head_tiles = (int)((group + 8 * nt - 1) / (8 * nt));
+  a.batch = (int)batch, a.lengths = lengths;
   a.most = weights && weights_width < tokens ? weights_width : tokens;
-  a.chunk = p.chunk, a.chunks = p.chunks;
-  const bool parts = p.chunks > 1 || weights != nullptr;
+  const bool parts = tokens > kUnit;  // otherwise every row is one unit and finished by its CTA
   a.part_ml = parts ? reinterpret_cast<float2 *>(ws + w.ml) : nullptr;
   a.part_o = parts ? reinterpret_cast<float *>(ws + w.o) : nullptr;
+  a.stats = weights ? reinterpret_cast<float2 *>(ws + w.stats) : nullptr;
   a.scores = weights ? reinterpret_cast<float *>(ws + w.scores) : nullptr;
   a.score_tokens = tokens;
   a.weights = weights, a.weights_width = weights_width, a.status = status;
   const Table t{page_table, table_stride, table_width};
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == MXQ_BF16)
-    launch_attention<__nv_bfloat16>(cache->format, dim, c, t, a, p, batch, st);
-  else
-    launch_attention<float>(cache->format, dim, c, t, a, p, batch, st);
-  if (cudaGetLastError() != cudaSuccess) return MXQ_ERR_LAUNCH;
-  if (!parts) return MXQ_OK;
-  const dim3 join_grid((unsigned)q_heads, (unsigned)batch);
-  if (dtype == MXQ_BF16)
-    join_kernel<__nv_bfloat16><<<join_grid, kJoinThreads, 0, st>>>(a, dim);
-  else
-    join_kernel<float><<<join_grid, kJoinThreads, 0, st>>>(a, dim);
-  if (cudaGetLastError() != cudaSuccess) return MXQ_ERR_LAUNCH;
-  if (weights) {
-    int64_t x = (tokens + kJoinThreads - 1) / kJoinThreads;
+  rc = dtype == MXQ_BF16 ? launch_attention<__nv_bfloat16>(cache->format, dim, c, t, a, nt, most_ctas, st)
+                         : launch_attention<float>(cache->format, dim, c, t, a, nt, most_ctas, st);
+  if (rc != MXQ_OK || (!parts && !weights)) return rc;
+  int64_t x = group;
+  if (weights) {  // enough CTAs for the tokens, and no more than the GPU holds at once
+    const int64_t need = (tokens + kFinishThreads - 1) / kFinishThreads;
     const int64_t cap = ((int64_t)gemm::sm_count() * 16 + c.heads * batch - 1) / (c.heads * batch);
-    if (x > cap) x = cap;
-    weights_kernel<<<dim3((unsigned)x, (unsigned)c.heads, (unsigned)batch), kJoinThreads, group * sizeof(float2), st>>>(
-        a, c.heads, 8 * p.nt);
-    if (cudaGetLastError() != cudaSuccess) return MXQ_ERR_LAUNCH;
+    x = need < cap ? need : cap;
   }
-  return MXQ_OK;
+  return dtype == MXQ_BF16 ? launch_finish<__nv_bfloat16>(a, c.heads, 8 * nt, dim, (unsigned)x, st)
+                           : launch_finish<float>(a, c.heads, 8 * nt, dim, (unsigned)x, st);
 }
 
 }  // extern "C"
