@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "mxq.h"
 #include "mxq_common.cuh"
 #include "mxq_internal.h"
@@ -553,10 +555,16 @@ int mxq_paged_evict(const mxq_paged_cache *cache, int64_t batch, const int32_t *
   const Table t{page_table, table_stride, table_width};
   cudaStream_t st = (cudaStream_t)stream;
   const int64_t n_keys = width < kKeysInShared ? width : kKeysInShared;
-  if (cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeysInShared * 4) !=
-      cudaSuccess) {
-    cudaGetLastError();
-    return MXQ_ERR_LAUNCH;
+  static std::atomic<bool> set_up[64];  // the kernel's shared memory limit has been raised on this device
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return MXQ_ERR_LAUNCH;
+  if (!set_up[device & 63].load(std::memory_order_relaxed)) {
+    if (cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kKeysInShared * 4) !=
+        cudaSuccess) {
+      cudaGetLastError();
+      return MXQ_ERR_LAUNCH;
+    }
+    set_up[device & 63].store(true, std::memory_order_relaxed);
   }
   evict_select_kernel<<<dim3((unsigned)c.heads, (unsigned)batch), kSelectThreads, (size_t)n_keys * 4, st>>>(
       c, table_width << c.page_log2, a);

@@ -20,6 +20,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "mxq.h"
 #include "mxq_common.cuh"
 #include "mxq_internal.h"
@@ -959,11 +961,17 @@ template <typename T, int kFormat, int D, int NT>
 static int launch_one(const Cache &c, const Table &t, AttnArgs &a, int64_t most_ctas, cudaStream_t st) {
   constexpr int kSmem = Smem<kFormat, D, NT>::kTotal;
   auto kernel = attention_kernel<T, kFormat, D, NT>;
-  int per_sm = 0;
-  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
-      cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kWarps * 32, kSmem) != cudaSuccess || per_sm < 1) {
-    cudaGetLastError();
-    return MXQ_ERR_LAUNCH;
+  static std::atomic<int> known[64];  // CTAs per SM on each device, once the kernel has been set up there
+  int device = 0;
+  if (cudaGetDevice(&device) != cudaSuccess) return MXQ_ERR_LAUNCH;
+  int per_sm = known[device & 63].load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem) != cudaSuccess ||
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kWarps * 32, kSmem) != cudaSuccess || per_sm < 1) {
+      cudaGetLastError();
+      return MXQ_ERR_LAUNCH;
+    }
+    known[device & 63].store(per_sm, std::memory_order_relaxed);
   }
   int64_t ctas = (int64_t)gemm::sm_count() * (per_sm < kMostPerSm ? per_sm : kMostPerSm);
   if (ctas > most_ctas) ctas = most_ctas;

@@ -117,9 +117,148 @@ at::Tensor mx_fake(const at::Tensor &x, int64_t kind, int64_t block, int64_t p0,
   return y;
 }
 
+// ---- paged key/value cache -------------------------------------------------------------------------------------------
+// The calls of mase_b200.kv_cache for arguments that need no copy and no complaint: everything else returns None (or
+// false) and is left to the Python functions, which check in detail, copy what must be copied and raise.
+
+bool on(const at::Tensor &t, int64_t device) { return t.is_cuda() && t.device().index() == device; }
+bool float_type(const at::Tensor &t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
+
+bool plain_table(const at::Tensor &table, const at::Tensor &lengths, int64_t device) {
+  return on(table, device) && on(lengths, device) && table.scalar_type() == at::kInt && lengths.scalar_type() == at::kInt &&
+         table.dim() == 2 && lengths.dim() == 1 && table.size(0) == lengths.size(0) && table.size(0) > 0 &&
+         table.size(1) > 0 && table.stride(1) == 1 && (table.size(0) == 1 || table.stride(0) >= table.size(1)) &&
+         lengths.is_contiguous();
+}
+bool plain_vector(const c10::optional<at::Tensor> &t, int64_t n, int64_t device) {
+  return !t.has_value() ||
+         (on(*t, device) && t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == n && t->is_contiguous());
+}
+bool plain_stats(const at::Tensor &t, at::ScalarType type, int64_t batch, int64_t heads, int64_t device) {
+  return on(t, device) && t.scalar_type() == type && t.dim() == 3 && t.size(0) == batch && t.size(1) == heads &&
+         t.size(2) > 0 && t.is_contiguous();
+}
+void *ptr(const c10::optional<at::Tensor> &t) { return t.has_value() ? t->data_ptr() : nullptr; }
+
+c10::optional<at::Tensor> paged_attention(int64_t cache, int64_t device, const at::Tensor &query, const at::Tensor &table,
+                                          const at::Tensor &lengths, double scaling, const c10::optional<at::Tensor> &weights,
+                                          const at::Tensor &status) {
+  const auto *c = reinterpret_cast<const mxq_paged_cache *>(cache);
+  const int64_t nd = query.dim();
+  if (!on(query, device) || !float_type(query) || (query.requires_grad() && at::GradMode::is_enabled()) ||
+      !plain_table(table, lengths, device) || (nd != 3 && nd != 4) || (nd == 4 && query.size(2) != 1) ||
+      query.size(0) != table.size(0) || query.size(nd - 1) != c->head_dim || query.stride(nd - 1) != 1 ||
+      query.size(1) < 1 || query.size(1) % c->heads != 0)
+    return c10::nullopt;
+  const int64_t batch = query.size(0), heads = query.size(1), width = table.size(1);
+  if (weights.has_value() && !plain_stats(*weights, at::kFloat, batch, c->heads, device)) return c10::nullopt;
+  const c10::cuda::CUDAGuard guard(query.device());
+  const int64_t n_ws = mxq_paged_attention_workspace_bytes(c, batch, heads, width, weights.has_value());
+  if (n_ws < 0) return c10::nullopt;
+  at::Tensor out = at::empty(query.sizes(), query.options());
+  at::Tensor ws = at::empty({n_ws}, query.options().dtype(at::kByte));
+  const int rc = mxq_paged_attention(
+      c, query.data_ptr(), out.data_ptr(), dtype_code(query.scalar_type()), batch, heads, query.stride(0), query.stride(1),
+      (float)scaling, static_cast<const int32_t *>(table.data_ptr()), width, table.stride(0),
+      static_cast<const int32_t *>(lengths.data_ptr()), static_cast<float *>(ptr(weights)),
+      weights.has_value() ? weights->size(2) : 0, ws.data_ptr(), n_ws, static_cast<int *>(status.data_ptr()),
+      at::cuda::getCurrentCUDAStream(device).stream());
+  check_rc(rc, "mxq_paged_attention");
+  return out;
+}
+
+// every row on a 16-byte boundary, the last dimension contiguous
+bool plain_rows(const at::Tensor &t) {
+  const int64_t need = 16 / t.element_size();
+  if (t.stride(3) != 1 || reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) return false;
+  for (int d = 0; d < 3; ++d)
+    if (t.size(d) > 1 && t.stride(d) % need) return false;
+  return true;
+}
+int64_t step(const at::Tensor &t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
+bool paged_append(int64_t cache, int64_t device, const at::Tensor &key, const at::Tensor &value, const at::Tensor &table,
+                  const at::Tensor &lengths, const c10::optional<at::Tensor> &counts,
+                  const c10::optional<at::Tensor> &positions, const c10::optional<at::Tensor> &next_position, int64_t tab,
+                  const at::Tensor &status) {
+  const auto *c = reinterpret_cast<const mxq_paged_cache *>(cache);
+  if (!on(key, device) || !on(value, device) || !float_type(key) || value.scalar_type() != key.scalar_type() ||
+      !plain_table(table, lengths, device) || key.dim() != 4 || key.sizes() != value.sizes() ||
+      key.size(0) != table.size(0) || key.size(1) != c->heads || key.size(3) != c->head_dim || key.numel() == 0 ||
+      !plain_rows(key) || !plain_rows(value))
+    return false;
+  const int64_t batch = key.size(0);
+  if (!plain_vector(counts, batch, device) || !plain_vector(next_position, batch, device) ||
+      (positions.has_value() ? !plain_stats(*positions, at::kInt, batch, c->heads, device) : next_position.has_value()))
+    return false;
+  const c10::cuda::CUDAGuard guard(key.device());
+  const int rc = mxq_paged_append(
+      c, key.data_ptr(), value.data_ptr(), dtype_code(key.scalar_type()), batch, key.size(2), step(key, 0), step(key, 1),
+      step(key, 2), step(value, 0), step(value, 1), step(value, 2), static_cast<const int32_t *>(table.data_ptr()),
+      table.size(1), table.stride(0), static_cast<const int32_t *>(lengths.data_ptr()),
+      static_cast<const int32_t *>(ptr(counts)), static_cast<int32_t *>(ptr(positions)),
+      positions.has_value() ? positions->size(2) : 0, static_cast<const int32_t *>(ptr(next_position)),
+      reinterpret_cast<const uint8_t *>(tab), static_cast<int *>(status.data_ptr()),
+      at::cuda::getCurrentCUDAStream(device).stream());
+  check_rc(rc, "mxq_paged_append");
+  return true;
+}
+
+c10::optional<std::tuple<at::Tensor, at::Tensor>> paged_gather(int64_t cache, int64_t device, const at::Tensor &table,
+                                                               const at::Tensor &lengths, int64_t max_length,
+                                                               at::ScalarType dtype, const at::Tensor &status) {
+  const auto *c = reinterpret_cast<const mxq_paged_cache *>(cache);
+  if (!plain_table(table, lengths, device) || max_length < 1 || (dtype != at::kFloat && dtype != at::kBFloat16))
+    return c10::nullopt;
+  const c10::cuda::CUDAGuard guard(table.device());
+  const int64_t batch = table.size(0);
+  at::Tensor key = at::empty({batch, c->heads, max_length, c->head_dim}, table.options().dtype(dtype));
+  at::Tensor value = at::empty_like(key);
+  const int rc = mxq_paged_gather(c, key.data_ptr(), value.data_ptr(), dtype_code(dtype), batch, max_length,
+                                  static_cast<const int32_t *>(table.data_ptr()), table.size(1), table.stride(0),
+                                  static_cast<const int32_t *>(lengths.data_ptr()), static_cast<int *>(status.data_ptr()),
+                                  at::cuda::getCurrentCUDAStream(device).stream());
+  check_rc(rc, "mxq_paged_gather");
+  return std::make_tuple(key, value);
+}
+
+c10::optional<std::tuple<at::Tensor, at::Tensor, at::Tensor>> paged_evict(
+    int64_t cache, int64_t device, const at::Tensor &table, const at::Tensor &lengths, const at::Tensor &weights,
+    int64_t keep, int64_t recent, const c10::optional<at::Tensor> &positions,
+    const c10::optional<at::Tensor> &next_position, const at::Tensor &status) {
+  const auto *c = reinterpret_cast<const mxq_paged_cache *>(cache);
+  if (!plain_table(table, lengths, device)) return c10::nullopt;
+  const int64_t batch = table.size(0);
+  if (!plain_stats(weights, at::kFloat, batch, c->heads, device) || keep < 1 || keep > INT32_MAX || recent < 0 ||
+      recent > keep || positions.has_value() != next_position.has_value() || !plain_vector(next_position, batch, device) ||
+      (positions.has_value() && (!plain_stats(*positions, at::kInt, batch, c->heads, device) ||
+                                 positions->size(2) != weights.size(2))))
+    return c10::nullopt;
+  const c10::cuda::CUDAGuard guard(weights.device());
+  const int64_t width = weights.size(2);
+  const int64_t n_ws = mxq_paged_evict_workspace_bytes(c, batch, width, keep);
+  if (n_ws < 0) return c10::nullopt;
+  at::Tensor new_lengths = at::empty_like(lengths), new_weights = at::empty_like(weights);
+  at::Tensor new_positions = at::empty(weights.sizes(), lengths.options());
+  at::Tensor ws = at::empty({n_ws}, weights.options().dtype(at::kByte));
+  const int rc = mxq_paged_evict(
+      c, batch, static_cast<const int32_t *>(table.data_ptr()), table.size(1), table.stride(0),
+      static_cast<const int32_t *>(lengths.data_ptr()), static_cast<const float *>(weights.data_ptr()),
+      static_cast<const int32_t *>(ptr(positions)), static_cast<const int32_t *>(ptr(next_position)), width, keep, recent,
+      static_cast<int32_t *>(new_lengths.data_ptr()), static_cast<float *>(new_weights.data_ptr()),
+      static_cast<int32_t *>(new_positions.data_ptr()), ws.data_ptr(), n_ws, static_cast<int *>(status.data_ptr()),
+      at::cuda::getCurrentCUDAStream(device).stream());
+  check_rc(rc, "mxq_paged_evict");
+  return std::make_tuple(new_lengths, new_weights, new_positions);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  m.def("paged_attention", &paged_attention, "attention of one new token per sequence over a paged cache");
+  m.def("paged_append", &paged_append, "quantize new keys and values into a paged cache");
+  m.def("paged_gather", &paged_gather, "the rows of a paged cache as dense tensors");
+  m.def("paged_evict", &paged_evict, "eviction from a paged cache by accumulated attention weight");
   m.def("mx_fake", &mx_fake, "MXFP / MXINT quantize-dequantize of a contiguous run of blocks");
   m.def("mx_linear", &mx_linear, "LinearMXFP forward on packed weights (mxq_mx_linear)");
   m.def("dense_linear", &dense_linear, "F.linear of quantized bf16 / fp32 operands (mxq_gemm_dense)");

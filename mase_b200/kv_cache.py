@@ -29,8 +29,26 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from .gemm import _CHECK_EVERY_CALL, _status, check_status
+from . import gemm
+from .gemm import _status, check_status
 from .quantizers import _DT, _ceil_tab_ptr, _floor_tab_ptr, _on_device, _require_cuda, _stream
+
+_BINDING = None
+
+
+def _binding():
+    """The compiled torch binding when it is built and has the cache's entries, else False (see mase_b200.gemm._ext)."""
+    global _BINDING
+    if _BINDING is None:
+        ext = gemm._ext()
+        _BINDING = ext if ext and hasattr(ext, "paged_attention") else False
+    return _BINDING
+
+
+def _check_every_call(cache) -> None:
+    if gemm._CHECK_EVERY_CALL:
+        check_status(cache.device)
+
 
 _MXFP_FORMATS = {(4, 3): _lib.CACHE_E4M3, (5, 2): _lib.CACHE_E5M2, (2, 1): _lib.CACHE_E2M1X2}
 _HEAD_DIMS, _PAGE_SIZES = (32, 64, 128, 256), (16, 32, 64, 128, 256)
@@ -127,7 +145,7 @@ class PagedKVCache:
         self.fmt, self.config = (None, None) if code == _lib.CACHE_BF16 else (fmt, dict(config))
         self.key, self.value, self.key_scales, self.value_scales = key, value, key_scales, value_scales
         self.num_pages, self.num_kv_heads, self.page_size = key.shape[:3]
-        self.head_dim, self.device = dim, key.device
+        self.head_dim, self.device, self._index = dim, key.device, key.device.index
         self._code, self._bits = code, bits
         ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
         self._desc = _lib.PagedCache(ptr(key), ptr(value), ptr(key_scales), ptr(value_scales), self.num_pages, code, bits,
@@ -136,6 +154,8 @@ class PagedKVCache:
 
     def _log2_tab(self, dtype: torch.dtype):
         if self._code == _lib.CACHE_BF16:
+            return 0
+        if dtype not in _DT:
             return 0
         return _ceil_tab_ptr(dtype) if self._code == _lib.CACHE_INT8 else _floor_tab_ptr()
 
@@ -194,6 +214,10 @@ def paged_kv_append(cache: PagedKVCache, key: Tensor, value: Tensor, page_table:
 
     `positions` (int32 [batch, num_kv_heads, width]) is the record of token positions that `paged_kv_evict` keeps: the
     entries of the new slots become next_position[b] + t (int32 [batch]; default: lengths[b] + t)."""
+    ext = _binding()
+    if ext and ext.paged_append(cache._addr, cache._index, key, value, page_table, lengths, counts, positions, next_position,
+                                cache._log2_tab(key.dtype), _status(cache.device)):
+        return _check_every_call(cache)
     _require_cuda(key, "paged_kv_append")
     _require_cuda(value, "paged_kv_append")
     if key.dtype not in _DT or value.dtype != key.dtype:
@@ -225,8 +249,7 @@ def paged_kv_append(cache: PagedKVCache, key: Tensor, value: Tensor, page_table:
             0 if next_position is None else next_position.data_ptr(), cache._log2_tab(key.dtype),
             _status(cache.device).data_ptr(), _stream(key))
     _lib.check(rc, "mxq_paged_append")
-    if _CHECK_EVERY_CALL:
-        check_status(cache.device)
+    _check_every_call(cache)
 
 
 def paged_kv_gather(cache: PagedKVCache, page_table: Tensor, lengths: Tensor, max_length: int,
@@ -234,6 +257,11 @@ def paged_kv_gather(cache: PagedKVCache, page_table: Tensor, lengths: Tensor, ma
     """The cached rows as dense tensors (key, value), each [batch, num_kv_heads, max_length, head_dim] of `dtype`: what
     `kv_cache_mxfp` / `kv_cache_mxint` made of the rows that went in.  Rows from lengths[b] on are zeros; tokens from
     max_length on are left out."""
+    ext = _binding()
+    if ext and (got := ext.paged_gather(cache._addr, cache._index, page_table, lengths, max_length, dtype,
+                                        _status(cache.device))) is not None:
+        _check_every_call(cache)
+        return got
     if dtype not in _DT:
         raise NotImplementedError(f"paged_kv_gather: dtype {dtype} is not supported (float32 and bfloat16 are)")
     batch = _check_table(cache, page_table, lengths)
@@ -248,8 +276,7 @@ def paged_kv_gather(cache: PagedKVCache, page_table: Tensor, lengths: Tensor, ma
                                          page_table.data_ptr(), page_table.shape[1], page_table.stride(0),
                                          lengths.data_ptr(), _status(cache.device).data_ptr(), _stream(key))
     _lib.check(rc, "mxq_paged_gather")
-    if _CHECK_EVERY_CALL:
-        check_status(cache.device)
+    _check_every_call(cache)
     return key, value
 
 
@@ -264,6 +291,13 @@ def paged_attention(cache: PagedKVCache, query: Tensor, page_table: Tensor, leng
 
     `weights` (fp32 [batch, num_kv_heads, width], width at least the largest length) accumulates in place: the softmax
     weight of every cached token, summed over the query heads of its key/value head, is added to its entry."""
+    if scaling is None:
+        scaling = cache.head_dim ** -0.5
+    ext = _binding()
+    if ext and (out := ext.paged_attention(cache._addr, cache._index, query, page_table, lengths, scaling, weights,
+                                           _status(cache.device))) is not None:
+        _check_every_call(cache)
+        return out
     _require_cuda(query, "paged_attention")
     if query.dtype not in _DT:
         raise NotImplementedError(f"paged_attention: dtype {query.dtype} is not supported (float32 and bfloat16 are)")
@@ -297,13 +331,12 @@ def paged_attention(cache: PagedKVCache, query: Tensor, page_table: Tensor, leng
         ws = torch.empty((n_ws,), dtype=torch.uint8, device=query.device)
         rc = lib.mxq_paged_attention(
             cache._addr, q.data_ptr(), out.data_ptr(), _DT[q.dtype], batch, heads, q.stride(0), q.stride(1),
-            cache.head_dim ** -0.5 if scaling is None else float(scaling), page_table.data_ptr(), width,
+            float(scaling), page_table.data_ptr(), width,
             page_table.stride(0), lengths.data_ptr(), 0 if weights is None else weights.data_ptr(),
             0 if weights is None else weights.shape[2], ws.data_ptr(), n_ws, _status(cache.device).data_ptr(),
             _stream(query))
     _lib.check(rc, "mxq_paged_attention")
-    if _CHECK_EVERY_CALL:
-        check_status(cache.device)
+    _check_every_call(cache)
     return out
 
 
@@ -322,6 +355,11 @@ def paged_kv_evict(cache: PagedKVCache, page_table: Tensor, lengths: Tensor, wei
 
     Returns (lengths, weights, positions) of the shrunken sequences as new tensors; entries behind the new length are 0
     and -1.  The pages behind ceil(length / page_size) are free."""
+    ext = _binding()
+    if ext and (got := ext.paged_evict(cache._addr, cache._index, page_table, lengths, weights, keep, recent, positions,
+                                       next_position, _status(cache.device))) is not None:
+        _check_every_call(cache)
+        return got
     _require_cuda(weights, "paged_kv_evict")
     batch = _check_table(cache, page_table, lengths)
     _check_stats(weights, "weights", torch.float32, batch, cache)
@@ -350,6 +388,5 @@ def paged_kv_evict(cache: PagedKVCache, page_table: Tensor, lengths: Tensor, wei
                                  new_lengths.data_ptr(), new_weights.data_ptr(), new_positions.data_ptr(), ws.data_ptr(),
                                  n_ws, _status(cache.device).data_ptr(), _stream(weights))
     _lib.check(rc, "mxq_paged_evict")
-    if _CHECK_EVERY_CALL:
-        check_status(cache.device)
+    _check_every_call(cache)
     return new_lengths, new_weights, new_positions

@@ -481,6 +481,30 @@ def test_captured_steps_follow_their_tensors_and_share_nothing():
     gemm.check_status()
 
 
+def test_calls_without_the_compiled_binding(monkeypatch):
+    """The same C calls through ctypes, arguments that need a copy among them."""
+    from mase_b200 import kv_cache
+
+    got = []
+    for binding in (kv_cache._binding(), False):
+        monkeypatch.setattr(kv_cache, "_BINDING", binding)
+        cache, table = make_cache("e4m3", 2, 64, 16, [40, 33], fill=0)
+        x = rows(2, 2, 40, 66, seed=3, dtype=torch.bfloat16).to(DEV)
+        k, v = x[..., 1:65], x[..., 2:].transpose(2, 3).contiguous().transpose(2, 3)  # unaligned rows, strided elements
+        positions = torch.zeros(2, 2, 48, dtype=torch.int32, device=DEV)
+        mb.paged_kv_append(cache, k, v, table, i32([0, 0]), counts=i32([40, 33]), positions=positions, next_position=i32([5, 0]))
+        w = torch.zeros(2, 2, 48, device=DEV)
+        q = rows(2, 4, 64, 2, seed=4, dtype=torch.float32).to(DEV)[..., 0]
+        out = mb.paged_attention(cache, q, table, i32([40, 33]), weights=w)
+        gathered = mb.paged_kv_gather(cache, table, i32([40, 33]), 41, torch.float32)
+        evicted = mb.paged_kv_evict(cache, table, i32([40, 33]), w, 20, 4, positions, i32([45, 33]))
+        got.append([positions, w, out, *gathered, *evicted, cache.key, cache.value, cache.key_scales, cache.value_scales])
+        assert torch.equal(gathered[0][0, :, :40].cpu(), fake(k[0].cpu().contiguous(), "e4m3").float())
+    gemm.check_status()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+
+
 def test_refusals():
     cfg = CONFIGS["e4m3"][1]
     cache, table = make_cache("e4m3", 2, 64, 16, [16, 16])
