@@ -423,7 +423,7 @@ int mxq_paged_cache_size(void);
 /* Quantizes new keys and values into the pages: token t < counts[b] (counts NULL: t < tokens) of key / value
  * [batch, heads, tokens, head_dim] goes to slot lengths[b] + t of sequence b, with the codes and shared exponents of
  * the plain quantizers.  Element strides (batch, head, token); the last dimension is contiguous and every row starts on
- * a 16-byte boundary.  positions (optional, int32 [batch, heads, positions_width] contiguous): the entry of every written
+ * a 16-byte boundary; tokens <= 2^26.  positions (optional, int32 [batch, heads, positions_width] contiguous): the entry of every written
  * slot becomes next_position[b] + t (next_position NULL: lengths[b] + t).  log2_tab_host: the floor table (MXFP) or the
  * ceil table of `dtype` (MXINT); unused for MXQ_CACHE_BF16. */
 int mxq_paged_append(const mxq_paged_cache *cache, const void *key, const void *value, int dtype, int64_t batch,
@@ -433,8 +433,8 @@ int mxq_paged_append(const mxq_paged_cache *cache, const void *key, const void *
                      int64_t positions_width, const int32_t *next_position, const uint8_t *log2_tab_host, int *status,
                      void *stream);
 
-/* The cached rows as dense tensors: key, value [batch, heads, max_tokens, head_dim] of `dtype`, contiguous; rows from
- * lengths[b] on are zeros. */
+/* The cached rows as dense tensors: key, value [batch, heads, max_tokens, head_dim] of `dtype`, contiguous, 32-byte
+ * aligned; rows from lengths[b] on are zeros.  max_tokens <= 2^26. */
 int mxq_paged_gather(const mxq_paged_cache *cache, void *key, void *value, int dtype, int64_t batch, int64_t max_tokens,
                      const int32_t *page_table, int64_t table_width, int64_t table_stride, const int32_t *lengths,
                      int *status, void *stream);
@@ -442,7 +442,7 @@ int mxq_paged_gather(const mxq_paged_cache *cache, void *key, void *value, int d
 /* Attention of one new token per sequence over the pages, split over the cache's length and joined:
  *   s_j = scaling * <q, k_j>,  out = sum_j softmax(s)_j v_j  over j < lengths[b]  (zeros for an empty sequence)
  * q, out: [batch, q_heads, head_dim] of `dtype`; q with element strides (batch, head) and a contiguous last dimension, out
- * contiguous.  q_heads is a multiple of heads: query heads h * g .. h * g + g - 1 read key/value head h.
+ * contiguous and 16-byte aligned.  q_heads is a multiple of heads: query heads h * g .. h * g + g - 1 read key/value head h.
  * weights (optional, fp32 [batch, heads, weights_width] contiguous): weights[b, h, j] += sum of softmax(s)_j over the
  * query heads of h.  workspace: 16-byte aligned, at least mxq_paged_attention_workspace_bytes(...) bytes, not shared with
  * a call that may run at the same time. */

@@ -31,16 +31,6 @@ struct AppendArgs {
   int *status;
 };
 
-__device__ __forceinline__ void load16(const __nv_bfloat16 *p, float (&v)[16]) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint4 r = reinterpret_cast<const uint4 *>(p)[i];
-    uint32_t b[8];
-    unpack(r, b);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[8 * i + k] = __uint_as_float(b[k]);
-  }
-}
 __device__ __forceinline__ void load16(const float *p, float (&v)[16]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -56,21 +46,42 @@ __device__ __forceinline__ uint4 bytes_of(const uint32_t (&c)[16]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Codes of this lane's 16 elements (one per byte) and the block's scale byte.  Every lane of the warp calls it.
-template <typename T, int kFormat>
-__device__ __forceinline__ uint4 encode16(const T *p, bool live, int bits, const Log2Tab &tab, int &scale) {
-  using Fmt = Format<kFormat>;
-  if constexpr (Elem<T>::kBf16) {
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    const uint4 lo = live ? reinterpret_cast<const uint4 *>(p)[0] : zero;
-    const uint4 hi = live ? reinterpret_cast<const uint4 *>(p)[1] : zero;
+// Half a block of 32 elements: loaded, and turned into codes (one per byte) and the block's scale byte together with the
+// neighbouring lane's half.  Every lane of the warp calls encode().
+template <typename T>
+struct Half;
+template <>
+struct Half<__nv_bfloat16> {
+  uint4 lo, hi;
+  __device__ __forceinline__ void clear() { lo = hi = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
+    lo = ld_stream(reinterpret_cast<const uint4 *>(p)), hi = ld_stream(reinterpret_cast<const uint4 *>(p) + 1);
+  }
+  __device__ __forceinline__ void store_bf16(uint4 *d) const { d[0] = lo, d[1] = hi; }
+  template <int kFormat>
+  __device__ __forceinline__ uint4 encode(int bits, const Log2Tab &tab, int &scale) const {
     if constexpr (kFormat == MXQ_CACHE_INT8)
       return mxint_codes_bf16(lo, hi, tab, bits, scale);
     else
-      return codes_bf16<Fmt::E, Fmt::F>(lo, hi, tab, scale);
-  } else {
-    float v[16] = {};
-    if (live) load16(p, v);
+      return codes_bf16<Format<kFormat>::E, Format<kFormat>::F>(lo, hi, tab, scale);
+  }
+};
+template <>
+struct Half<float> {
+  float v[16];
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = 0.f;
+  }
+  __device__ __forceinline__ void load(const float *p) { load16(p, v); }
+  __device__ __forceinline__ void store_bf16(uint4 *d) const {
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      d[k] = make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
+                        pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+  }
+  template <int kFormat>
+  __device__ __forceinline__ uint4 encode(int bits, const Log2Tab &tab, int &scale) const {
     uint32_t code[16];
     if constexpr (kFormat == MXQ_CACHE_INT8) {
       float amax = 0.f;
@@ -82,6 +93,7 @@ __device__ __forceinline__ uint4 encode16(const T *p, bool live, int bits, const
 #pragma unroll
       for (int k = 0; k < 16; ++k) code[k] = (uint32_t)(int)mxint_mant(v[k], b);
     } else {
+      using Fmt = Format<kFormat>;
       uint32_t amax = 0;
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
@@ -99,16 +111,20 @@ __device__ __forceinline__ uint4 encode16(const T *p, bool live, int bits, const
     }
     return bytes_of(code);
   }
-}
+};
 
-// grid: (chunks of the units of one (sequence, head), heads * 2 sides, batch); a unit is half a block of one token.
+// grid: (chunks of the units of one (sequence, head), heads * 2 sides, batch); a unit is half a block of one token, and a
+// thread has two in flight: the reads of the rows and of the page table do not depend on one another.
 template <typename T, int kFormat>
-__global__ void __launch_bounds__(kThreads)
-append_kernel(const Cache c, const Table table, const AppendArgs a, int dim, const __grid_constant__ Log2Tab tab) {
+__global__ void __launch_bounds__(kThreads, Elem<T>::kBf16 ? 4 : 2)
+append_kernel(const Cache c, const Table table, const AppendArgs a, int dim_log2, const __grid_constant__ Log2Tab tab) {
   using Fmt = Format<kFormat>;
-  const int side = blockIdx.y & 1, head = blockIdx.y >> 1;
+  constexpr int kAtOnce = 2;
+  wait_for_previous();
+  let_next_start();
+  const int side = blockIdx.y & 1, head = blockIdx.y >> 1, dim = 1 << dim_log2;
   const int64_t b = blockIdx.z;
-  const int units = dim >> 4;  // 2, 4, 8 or 16: a pair of lanes never straddles two rows
+  const int units_log2 = dim_log2 - 4;  // 2, 4, 8 or 16 units a token: a pair of lanes never straddles two rows
   const int64_t most = table.width << c.page_log2;
   const int length = clamp_length(a.lengths[b], most, a.status);
   int64_t count = a.counts != nullptr ? a.counts[b] : a.tokens;
@@ -116,129 +132,167 @@ append_kernel(const Cache c, const Table table, const AppendArgs a, int dim, con
     report(a.status);
     count = count < 0 ? 0 : min(min(count, a.tokens), most - length);
   }
-  const T *src = static_cast<const T *>(a.src[side]) + b * a.stride_b[side] + head * a.stride_h[side];
-  const int64_t total = count * units;
-  const int64_t step = (int64_t)gridDim.x * kThreads;
-  for (int64_t base = (int64_t)blockIdx.x * kThreads; base < total; base += step) {
-    const int64_t i = base + threadIdx.x;
-    const bool live = i < total;
-    const int64_t t = live ? i / units : 0;
-    const int u = (int)(i - t * units);
-    int64_t row = -1;
-    int slot = 0;
-    if (live) {
-      slot = length + (int)t;
-      row = page_row(c, table, b, head, slot, a.status);
-      if (row >= 0) row += slot & ((1 << c.page_log2) - 1);
-    }
-    const T *p = src + t * a.stride_t[side] + u * 16;
-    if constexpr (kFormat == MXQ_CACHE_BF16) {
-      if (row >= 0) {
-        uint4 *d = reinterpret_cast<uint4 *>(c.codes[side] + row * (dim * 2) + u * 32);
-        if constexpr (Elem<T>::kBf16) {
-          d[0] = reinterpret_cast<const uint4 *>(p)[0], d[1] = reinterpret_cast<const uint4 *>(p)[1];
-        } else {
-          float v[16];
-          load16(p, v);
+  const int64_t stride_t = side ? a.stride_t[1] : a.stride_t[0];
+  const T *src = static_cast<const T *>(side ? a.src[1] : a.src[0]) + b * (side ? a.stride_b[1] : a.stride_b[0]) +
+                 head * (side ? a.stride_h[1] : a.stride_h[0]);
+  uint8_t *codes = side ? c.codes[1] : c.codes[0], *scales = side ? c.scales[1] : c.scales[0];
+  const int total = (int)count << units_log2;  // at most 2^26 tokens of 16 units
+  const int step = gridDim.x * (kThreads * kAtOnce);
+  for (int base = blockIdx.x * (kThreads * kAtOnce); base < total; base += step) {
+    int64_t row[kAtOnce];
+    Half<T> raw[kAtOnce];
 #pragma unroll
-          for (int k = 0; k < 2; ++k)
-            d[k] = make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                              pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7]));
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int i = base + k * kThreads + threadIdx.x, t = i >> units_log2, u = i & ((1 << units_log2) - 1);
+      row[k] = -1;
+      raw[k].clear();
+      if (i < total) {
+        raw[k].load(src + t * stride_t + u * 16);
+        const int slot = length + t;
+        row[k] = page_row(c, table, b, head, slot, a.status);
+        if (row[k] >= 0) row[k] += slot & ((1 << c.page_log2) - 1);
+        if (side == 0 && u == 0 && a.positions != nullptr) {
+          if (slot < a.positions_width)
+            a.positions[(b * c.heads + head) * a.positions_width + slot] =
+                (a.next_position != nullptr ? a.next_position[b] : length) + t;
+          else
+            report(a.status);
         }
       }
-    } else {
-      int scale;
-      const uint4 code = encode16<T, kFormat>(p, live, c.bits, tab, scale);
-      if (row >= 0) {
-        if constexpr (Fmt::kBits == 4) {
-          uint32_t w[4] = {code.x, code.y, code.z, code.w};
-#pragma unroll
-          for (int k = 0; k < 4; ++k) w[k] |= w[k] >> 4;  // bytes 0 and 2 now hold two codes each
-          *reinterpret_cast<uint2 *>(c.codes[side] + row * (dim / 2) + u * 8) =
-              make_uint2(__byte_perm(w[0], w[1], 0x6420), __byte_perm(w[2], w[3], 0x6420));
-        } else {
-          *reinterpret_cast<uint4 *>(c.codes[side] + row * dim + u * 16) = code;
-        }
-        if ((u & 1) == 0) c.scales[side][row * (dim >> 5) + (u >> 1)] = (uint8_t)scale;
-      }
     }
-    if (side == 0 && u == 0 && live && a.positions != nullptr) {
-      if (slot < a.positions_width)
-        a.positions[(b * c.heads + head) * a.positions_width + slot] =
-            (a.next_position != nullptr ? a.next_position[b] : length) + (int)t;
-      else
-        report(a.status);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int u = (base + k * kThreads + threadIdx.x) & ((1 << units_log2) - 1);
+      if constexpr (kFormat == MXQ_CACHE_BF16) {
+        if (row[k] >= 0) raw[k].store_bf16(reinterpret_cast<uint4 *>(codes + row[k] * (dim * 2) + u * 32));
+      } else {
+        int scale;
+        const uint4 code = raw[k].template encode<kFormat>(c.bits, tab, scale);
+        if (row[k] >= 0) {
+          if constexpr (Fmt::kBits == 4) {
+            uint32_t w[4] = {code.x, code.y, code.z, code.w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) w[x] |= w[x] >> 4;  // bytes 0 and 2 now hold two codes each
+            *reinterpret_cast<uint2 *>(codes + row[k] * (dim / 2) + u * 8) =
+                make_uint2(__byte_perm(w[0], w[1], 0x6420), __byte_perm(w[2], w[3], 0x6420));
+          } else {
+            *reinterpret_cast<uint4 *>(codes + row[k] * dim + u * 16) = code;
+          }
+          if ((u & 1) == 0) scales[row[k] * (dim >> 5) + (u >> 1)] = (uint8_t)scale;
+        }
+      }
     }
   }
 }
 
 // ---- gather ----------------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void store16(__nv_bfloat16 *p, const float (&v)[16]) {
-#pragma unroll
-  for (int k = 0; k < 2; ++k)
-    st_stream(reinterpret_cast<uint4 *>(p) + k,
-              make_uint4(pack_bf16x2(v[8 * k], v[8 * k + 1]), pack_bf16x2(v[8 * k + 2], v[8 * k + 3]),
-                         pack_bf16x2(v[8 * k + 4], v[8 * k + 5]), pack_bf16x2(v[8 * k + 6], v[8 * k + 7])));
-}
-__device__ __forceinline__ void store16(float *p, const float (&v)[16]) {
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    st_stream(reinterpret_cast<uint4 *>(p) + k,
-              make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]),
-                         __float_as_uint(v[4 * k + 3])));
+// 32 bytes, aligned to 32
+__device__ __forceinline__ void store32(void *p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.cs.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]),
+               "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
 }
 
-// 16 elements from `p` (codes) with the block's scale byte.
-template <int kFormat>
-__device__ __forceinline__ void decode16(const uint8_t *p, int scale, int bits, float (&v)[16]) {
-  using Fmt = Format<kFormat>;
+// 16 elements of a block as 8 bf16 pairs in order.  The values are codes times a power of two: exact in bf16 unless the
+// block's scale lies at an end of the range (kRare), where the second factor or the rounding to subnormals takes part.
+template <int kFormat, bool kRare>
+__device__ __forceinline__ void decode16(const uint8_t *p, uint32_t scale, int bits, uint32_t (&out)[8]) {
   if constexpr (kFormat == MXQ_CACHE_BF16) {
-    load16(reinterpret_cast<const __nv_bfloat16 *>(p), v);
-  } else if constexpr (Fmt::kBits == 4) {
-    const uint2 r = *reinterpret_cast<const uint2 *>(p);
-    const float sf = pow2f(scale - 127);
-#pragma unroll
-    for (int k = 0; k < 16; ++k)
-      v[k] = mxfp_decode(((k < 8 ? r.x : r.y) >> (4 * (k & 7))) & 15u, Fmt::E, Fmt::F) * sf;
+    const uint4 lo = ld_stream(reinterpret_cast<const uint4 *>(p)), hi = ld_stream(reinterpret_cast<const uint4 *>(p) + 1);
+    out[0] = lo.x, out[1] = lo.y, out[2] = lo.z, out[3] = lo.w, out[4] = hi.x, out[5] = hi.y, out[6] = hi.z, out[7] = hi.w;
   } else {
-    const uint4 r = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-    const float sf = kFormat == MXQ_CACHE_INT8 ? (scale == 255 ? INFINITY : pow2f(scale - 127 - (bits - 1)))
-                                               : pow2f(scale - 127);
+    const int offset = raw_offset<kFormat>(bits);
+    const uint32_t f = kRare ? rare_factor<kFormat>(scale, offset) * 0x00010001u : (uint32_t)((int)scale + offset) * 0x00800080u;
+    const uint32_t rest = kRare ? rare_rest<kFormat>(scale, offset) * 0x00010001u : 0u;
+    uint32_t e[8];
+    if constexpr (Format<kFormat>::kBits == 4) {
+      const uint2 r = __ldcs(reinterpret_cast<const uint2 *>(p));
+      key_word<kFormat, kRare>(r.x, f, rest, e), key_word<kFormat, kRare>(r.y, f, rest, e + 4);
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const uint32_t code = (w[k >> 2] >> (8 * (k & 3))) & 0xFFu;
-      v[k] = (kFormat == MXQ_CACHE_INT8 ? (float)(int8_t)code : mxfp_decode(code, Fmt::E, Fmt::F)) * sf;
+      for (int k = 0; k < 2; ++k) {  // (0, 2) (4, 6) (1, 3) (5, 7) -> (0, 1) (2, 3) (4, 5) (6, 7)
+        out[4 * k] = __byte_perm(e[4 * k], e[4 * k + 2], 0x5410), out[4 * k + 1] = __byte_perm(e[4 * k], e[4 * k + 2], 0x7632);
+        out[4 * k + 2] = __byte_perm(e[4 * k + 1], e[4 * k + 3], 0x5410);
+        out[4 * k + 3] = __byte_perm(e[4 * k + 1], e[4 * k + 3], 0x7632);
+      }
+    } else {
+      const uint4 r = ld_stream(reinterpret_cast<const uint4 *>(p));
+      const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (kFormat == MXQ_CACHE_INT8) {  // (0, 2) (1, 3) -> (0, 1) (2, 3)
+          key_word<kFormat, kRare>(w[k], f, rest, e);
+          out[2 * k] = __byte_perm(e[0], e[1], 0x5410), out[2 * k + 1] = __byte_perm(e[0], e[1], 0x7632);
+        } else {
+          key_word<kFormat, kRare>(w[k], f, rest, &out[2 * k]);
+        }
+      }
     }
+  }
+}
+// The same in fp32, from the element codecs: for scales at which a product may be below the range of bf16.
+template <int kFormat>
+__device__ __forceinline__ void decode16_wide(const uint8_t *p, int scale, int bits, float (&v)[16]) {
+  using Fmt = Format<kFormat>;
+  const float sf = kFormat == MXQ_CACHE_INT8 ? (scale == 255 ? INFINITY : pow2f(scale - 127 - (bits - 1))) : pow2f(scale - 127);
+#pragma unroll
+  for (int k = 0; k < 16; ++k) {
+    const uint32_t code = Fmt::kBits == 4 ? (p[k >> 1] >> (4 * (k & 1))) & 15u : p[k];
+    v[k] = (kFormat == MXQ_CACHE_INT8 ? (float)(int8_t)code : mxfp_decode(code, Fmt::E, Fmt::F)) * sf;
   }
 }
 
 // grid: (chunks of the units of one (sequence, head), heads * 2 sides, batch); a unit is 16 elements of one token.
 template <typename T, int kFormat>
 __global__ void __launch_bounds__(kThreads)
-gather_kernel(const Cache c, const Table table, const int32_t *lengths, T *key, T *value, int64_t tokens, int dim,
+gather_kernel(const Cache c, const Table table, const int32_t *lengths, T *key, T *value, int64_t tokens, int dim_log2,
               int *status) {
   using Fmt = Format<kFormat>;
-  const int side = blockIdx.y & 1, head = blockIdx.y >> 1;
+  wait_for_previous();
+  let_next_start();
+  const int side = blockIdx.y & 1, head = blockIdx.y >> 1, dim = 1 << dim_log2;
   const int64_t b = blockIdx.z;
-  const int units = dim >> 4;
+  const int units_log2 = dim_log2 - 4;
   const int length = clamp_length(lengths[b], table.width << c.page_log2, status);
+  const uint8_t *codes = side ? c.codes[1] : c.codes[0], *scales = side ? c.scales[1] : c.scales[0];
   T *dst = (side ? value : key) + (b * c.heads + head) * tokens * dim;
-  const int64_t total = tokens * units;
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-    const int64_t t = i / units;
-    const int u = (int)(i - t * units);
-    float v[16] = {};
-    if (t < length) {
-      int64_t row = page_row(c, table, b, head, (int)t, status);
-      if (row >= 0) {
-        row += t & ((1 << c.page_log2) - 1);
-        int scale = 0;
-        if constexpr (kFormat != MXQ_CACHE_BF16) scale = c.scales[side][row * (dim >> 5) + (u >> 1)];
-        decode16<kFormat>(c.codes[side] + row * (dim * Fmt::kBits / 8) + u * (2 * Fmt::kBits), scale, c.bits, v);
+  const int total = (int)tokens << units_log2;  // at most 2^26 tokens of 16 units
+#pragma unroll 2
+  for (int i = blockIdx.x * kThreads + threadIdx.x; i < total; i += gridDim.x * kThreads) {
+    const int t = i >> units_log2, u = i & ((1 << units_log2) - 1);
+    int64_t row = -1;
+    if (t < length) row = page_row(c, table, b, head, t, status);
+    uint32_t w[8] = {};
+    T *to = dst + (int64_t)t * dim + u * 16;
+    if (row >= 0) {
+      row += t & ((1 << c.page_log2) - 1);
+      const uint8_t *p = codes + row * (dim * Fmt::kBits / 8) + u * (2 * Fmt::kBits);
+      uint32_t scale = 0;
+      if constexpr (kFormat != MXQ_CACHE_BF16) scale = scales[row * (dim >> 5) + (u >> 1)];
+      if constexpr (kFormat != MXQ_CACHE_BF16) {
+        if (!Elem<T>::kBf16 && scale < 16) {
+          float v[16];
+          decode16_wide<kFormat>(p, (int)scale, c.bits, v);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) store_scalar(to + k, v[k]);
+          continue;
+        }
       }
+      if (kFormat != MXQ_CACHE_BF16 && rare_scale<kFormat>(scale, raw_offset<kFormat>(c.bits)))
+        decode16<kFormat, true>(p, scale, c.bits, w);
+      else
+        decode16<kFormat, false>(p, scale, c.bits, w);
     }
-    store16(dst + t * dim + u * 16, v);
+    if constexpr (Elem<T>::kBf16) {
+      store32(to, w);
+    } else {
+      uint32_t lo[8], hi[8];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        lo[2 * k] = w[k] << 16, lo[2 * k + 1] = w[k] & 0xFFFF0000u;
+        hi[2 * k] = w[k + 4] << 16, hi[2 * k + 1] = w[k + 4] & 0xFFFF0000u;
+      }
+      store32(to, lo), store32(to + 8, hi);
+    }
   }
 }
 
@@ -288,6 +342,8 @@ __device__ __forceinline__ int scan_warps(int v, int *scratch, int &total) {
 
 __global__ void __launch_bounds__(kSelectThreads)
 evict_select_kernel(const Cache c, int64_t table_tokens, const EvictArgs a) {
+  wait_for_previous();
+  let_next_start();
   extern __shared__ uint32_t keys[];
   __shared__ int hist[kBins];
   __shared__ int scratch[32];
@@ -315,8 +371,14 @@ evict_select_kernel(const Cache c, int64_t table_tokens, const EvictArgs a) {
     return pos >= first_safe ? 0xFFFFFFFFu : key_of(w[j]);
   };
   auto key_at = [&](int j) { return shared_keys ? keys[j] : make_key(j); };
-  if (shared_keys)
-    for (int j = tid; j < n; j += kSelectThreads) keys[j] = make_key(j);
+  // every slot below `keep` starts out with its own statistics; the move kernel overwrites those that are filled anew
+#pragma unroll 8
+  for (int j = tid; j < n; j += kSelectThreads) {
+    const float x = w[j];
+    const int pos = p != nullptr ? p[j] : j;
+    if (j < m) nw[j] = x, np[j] = pos;
+    if (shared_keys) keys[j] = pos >= first_safe ? 0xFFFFFFFFu : key_of(x);
+  }
 
   uint32_t prefix = 0;  // the digits found so far, in place
   int need = m;         // how many of the keys that share the prefix are kept
@@ -386,46 +448,67 @@ evict_select_kernel(const Cache c, int64_t table_tokens, const EvictArgs a) {
     const uint32_t hb = __ballot_sync(0xFFFFFFFFu, hole), mb = __ballot_sync(0xFFFFFFFFu, mover);
     if (hole) to[hole_at + __popc(hb & below)] = j;
     if (mover) from[mover_at + __popc(mb & below)] = j;
-    if (kept && j < m) nw[j] = w[j], np[j] = p != nullptr ? p[j] : j;
     hole_at += __popc(hb), mover_at += __popc(mb);
-  }
-  __syncthreads();  // the lists are complete for the whole CTA
-  for (int i = tid; i < n_moves; i += kSelectThreads) {
-    const int s = from[i], d = to[i];
-    nw[d] = w[s], np[d] = p != nullptr ? p[s] : s;
   }
   if (tid == 0) a.moves[row] = n_moves;
 }
 
-// One warp per moved token: its key and value rows in 16-byte pieces, then the scale bytes.  Sources lie at or above
+// A warp takes 32 moves at a time: each lane looks one of them up (slots, pages) and moves its statistics, then the warp
+// copies the key and value rows of all of them, 16 bytes a lane with four copies in flight.  Sources lie at or above
 // `keep`, destinations below it, so moves never overlap.
 __global__ void __launch_bounds__(kThreads)
-evict_move_kernel(const Cache c, const Table table, const int32_t *from, const int32_t *to, const int32_t *moves,
-                  int max_moves, int row_bytes, int scale_bytes, int *status) {
+evict_move_kernel(const Cache c, const Table table, const EvictArgs a, int row_bytes_log2, int scale_bytes) {
+  wait_for_previous();
+  let_next_start();
   const int head = blockIdx.y, lane = threadIdx.x & 31;
   const int64_t b = blockIdx.z;
   const int64_t row = b * c.heads + head;
-  const int n = moves[row];
+  const int n = a.moves[row];
   const int in_page = (1 << c.page_log2) - 1;
-  const int pieces = row_bytes >> 4;
-  for (int i = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < n; i += gridDim.x * (kThreads / 32)) {
-    const int s = from[row * max_moves + i], d = to[row * max_moves + i];
-    int64_t sr = page_row(c, table, b, head, s, status), dr = page_row(c, table, b, head, d, status);
-    if (sr < 0 || dr < 0) continue;
-    sr += s & in_page, dr += d & in_page;
-    for (int k = lane; k < 2 * pieces; k += 32) {
-      const int side = k >= pieces, at = side ? k - pieces : k;
-      reinterpret_cast<uint4 *>(c.codes[side] + dr * row_bytes)[at] =
-          reinterpret_cast<const uint4 *>(c.codes[side] + sr * row_bytes)[at];
+  const int32_t *from = a.from + row * a.max_moves, *to = a.to + row * a.max_moves;
+  const int pieces_log2 = row_bytes_log2 - 4, pieces = 1 << pieces_log2;  // of 16 bytes
+  const int warps = gridDim.x * (kThreads / 32);
+  for (int i0 = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * 32; i0 < n; i0 += warps * 32) {
+    int64_t sr = -1, dr = -1;
+    if (i0 + lane < n) {
+      const int s = from[i0 + lane], d = to[i0 + lane];
+      a.new_weights[row * a.width + d] = a.weights[row * a.width + s];
+      a.new_positions[row * a.width + d] = a.positions != nullptr ? a.positions[row * a.width + s] : s;
+      sr = page_row(c, table, b, head, s, a.status), dr = page_row(c, table, b, head, d, a.status);
+      if (sr < 0 || dr < 0)
+        sr = dr = -1;
+      else
+        sr += s & in_page, dr += d & in_page;
     }
-    if (lane < 2 * scale_bytes) {
-      const int side = lane >= scale_bytes, at = side ? lane - scale_bytes : lane;
-      c.scales[side][dr * scale_bytes + at] = c.scales[side][sr * scale_bytes + at];
+    const int live = min(n - i0, 32);
+    // 16-byte pieces of the moves in order: [move][side][piece]
+    const int total = live << (pieces_log2 + 1);
+    for (int k0 = 0; k0 < total; k0 += 128) {
+      uint4 v[4];
+      uint8_t *dst[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int k = k0 + x * 32 + lane, move = min(k >> (pieces_log2 + 1), 31);
+        const int64_t ms = __shfl_sync(0xFFFFFFFFu, sr, move), md = __shfl_sync(0xFFFFFFFFu, dr, move);
+        uint8_t *side = (k >> pieces_log2) & 1 ? c.codes[1] : c.codes[0];
+        const int at = (k & (pieces - 1)) * 16;
+        dst[x] = nullptr;
+        if (k < total && ms >= 0) {
+          v[x] = ld_stream(reinterpret_cast<const uint4 *>(side + (ms << row_bytes_log2) + at));
+          dst[x] = side + (md << row_bytes_log2) + at;
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (dst[x] != nullptr) *reinterpret_cast<uint4 *>(dst[x]) = v[x];
     }
+    if (sr >= 0)
+      for (int k = 0; k < scale_bytes; ++k) {
+        c.scales[0][dr * scale_bytes + k] = c.scales[0][sr * scale_bytes + k];
+        c.scales[1][dr * scale_bytes + k] = c.scales[1][sr * scale_bytes + k];
+      }
   }
 }
-
-static int launched() { return cudaGetLastError() == cudaSuccess ? MXQ_OK : MXQ_ERR_LAUNCH; }
 
 // CTAs along x so that the whole grid holds about `per_sm` CTAs per SM, and no more than the work needs.
 static unsigned grid_x(int64_t need, int64_t yz, int per_sm) {
@@ -455,7 +538,7 @@ int mxq_paged_append(const mxq_paged_cache *cache, const void *key, const void *
   int rc = read_cache(cache, c);
   if (rc != MXQ_OK) return rc;
   if (dtype != MXQ_F32 && dtype != MXQ_BF16) return MXQ_ERR_DTYPE;
-  if (batch < 0 || tokens < 0 || tokens > INT32_MAX) return MXQ_ERR_SHAPE;
+  if (batch < 0 || tokens < 0 || tokens > (1 << 26)) return MXQ_ERR_SHAPE;
   if (batch == 0 || tokens == 0) return MXQ_OK;
   if ((rc = read_table(page_table, table_width, table_stride, batch, c.page_log2)) != MXQ_OK) return rc;
   if (!key || !value || !lengths || (!log2_tab_host && cache->format != MXQ_CACHE_BF16)) return MXQ_ERR_NULL;
@@ -475,18 +558,16 @@ int mxq_paged_append(const mxq_paged_cache *cache, const void *key, const void *
   const Table t{page_table, table_stride, table_width};
   const int dim = cache->head_dim;
   const int64_t yz = (int64_t)c.heads * 2 * batch;
-  const dim3 grid(grid_x((tokens * (dim / 16) + kThreads - 1) / kThreads, yz, 16), c.heads * 2, (unsigned)batch);
+  const dim3 grid(grid_x((tokens * (dim / 16) + 2 * kThreads - 1) / (2 * kThreads), yz, 4), c.heads * 2, (unsigned)batch);
   cudaStream_t st = (cudaStream_t)stream;
-#define CALL(f)                                                                               \
-  if (cache->format == f) {                                                                   \
-    if (dtype == MXQ_BF16)                                                                    \
-      append_kernel<__nv_bfloat16, f><<<grid, kThreads, 0, st>>>(c, t, a, dim, tab);          \
-    else                                                                                      \
-      append_kernel<float, f><<<grid, kThreads, 0, st>>>(c, t, a, dim, tab);                  \
-  }
+#define CALL(f)                                                                                                            \
+  if (cache->format == f)                                                                                                  \
+    return dtype == MXQ_BF16                                                                                               \
+               ? launch_chained(append_kernel<__nv_bfloat16, f>, grid, kThreads, 0, st, c, t, a, log2_of(dim), tab)        \
+               : launch_chained(append_kernel<float, f>, grid, kThreads, 0, st, c, t, a, log2_of(dim), tab);
   MXQ_PAGED_FORMATS(CALL)
 #undef CALL
-  return launched();
+  return MXQ_ERR_FORMAT;
 }
 
 int mxq_paged_gather(const mxq_paged_cache *cache, void *key, void *value, int dtype, int64_t batch, int64_t max_tokens,
@@ -496,28 +577,25 @@ int mxq_paged_gather(const mxq_paged_cache *cache, void *key, void *value, int d
   int rc = read_cache(cache, c);
   if (rc != MXQ_OK) return rc;
   if (dtype != MXQ_F32 && dtype != MXQ_BF16) return MXQ_ERR_DTYPE;
-  if (batch < 0 || max_tokens < 0 || max_tokens > INT32_MAX) return MXQ_ERR_SHAPE;
+  if (batch < 0 || max_tokens < 0 || max_tokens > (1 << 26)) return MXQ_ERR_SHAPE;
   if (batch == 0 || max_tokens == 0) return MXQ_OK;
   if ((rc = read_table(page_table, table_width, table_stride, batch, c.page_log2)) != MXQ_OK) return rc;
   if (!key || !value || !lengths) return MXQ_ERR_NULL;
-  if (!aligned(key, 16) || !aligned(value, 16)) return MXQ_ERR_ALIGN;
+  if (!aligned(key, 32) || !aligned(value, 32)) return MXQ_ERR_ALIGN;
   const Table t{page_table, table_stride, table_width};
   const int dim = cache->head_dim;
   const int64_t yz = (int64_t)c.heads * 2 * batch;
-  const dim3 grid(grid_x((max_tokens * (dim / 16) + kThreads - 1) / kThreads, yz, 16), c.heads * 2, (unsigned)batch);
+  const dim3 grid(grid_x((max_tokens * (dim / 16) + kThreads - 1) / kThreads, yz, 8), c.heads * 2, (unsigned)batch);
   cudaStream_t st = (cudaStream_t)stream;
-#define CALL(f)                                                                                                    \
-  if (cache->format == f) {                                                                                        \
-    if (dtype == MXQ_BF16)                                                                                         \
-      gather_kernel<__nv_bfloat16, f><<<grid, kThreads, 0, st>>>(c, t, lengths, (__nv_bfloat16 *)key,               \
-                                                                 (__nv_bfloat16 *)value, max_tokens, dim, status); \
-    else                                                                                                           \
-      gather_kernel<float, f><<<grid, kThreads, 0, st>>>(c, t, lengths, (float *)key, (float *)value, max_tokens,   \
-                                                         dim, status);                                             \
-  }
+#define CALL(f)                                                                                                             \
+  if (cache->format == f)                                                                                                   \
+    return dtype == MXQ_BF16 ? launch_chained(gather_kernel<__nv_bfloat16, f>, grid, kThreads, 0, st, c, t, lengths,        \
+                                              (__nv_bfloat16 *)key, (__nv_bfloat16 *)value, max_tokens, log2_of(dim), status) \
+                             : launch_chained(gather_kernel<float, f>, grid, kThreads, 0, st, c, t, lengths, (float *)key,  \
+                                              (float *)value, max_tokens, log2_of(dim), status);
   MXQ_PAGED_FORMATS(CALL)
 #undef CALL
-  return launched();
+  return MXQ_ERR_FORMAT;
 }
 
 static int64_t max_moves_of(int64_t width, int64_t keep) {
@@ -566,14 +644,13 @@ int mxq_paged_evict(const mxq_paged_cache *cache, int64_t batch, const int32_t *
     }
     set_up[device & 63].store(true, std::memory_order_relaxed);
   }
-  evict_select_kernel<<<dim3((unsigned)c.heads, (unsigned)batch), kSelectThreads, (size_t)n_keys * 4, st>>>(
-      c, table_width << c.page_log2, a);
-  if ((rc = launched()) != MXQ_OK || most == 0) return rc;
+  rc = launch_chained(evict_select_kernel, dim3((unsigned)c.heads, (unsigned)batch), kSelectThreads, (size_t)n_keys * 4, st, c,
+                      table_width << c.page_log2, a);
+  if (rc != MXQ_OK || most == 0) return rc;
   const int row_bytes = row_bytes_of(cache->format, cache->head_dim);
   const int scale_bytes = cache->format == MXQ_CACHE_BF16 ? 0 : cache->head_dim / 32;
-  const dim3 grid(grid_x((most + kThreads / 32 - 1) / (kThreads / 32), rows, 16), (unsigned)c.heads, (unsigned)batch);
-  evict_move_kernel<<<grid, kThreads, 0, st>>>(c, t, a.from, a.to, a.moves, a.max_moves, row_bytes, scale_bytes, status);
-  return launched();
+  const dim3 grid(grid_x((most + kThreads - 1) / kThreads, rows, 8), (unsigned)c.heads, (unsigned)batch);
+  return launch_chained(evict_move_kernel, grid, kThreads, 0, st, c, t, a, log2_of(row_bytes), scale_bytes);
 }
 
 }  // extern "C"

@@ -58,140 +58,6 @@ struct AttnArgs {
   int *status;
 };
 
-// ---- codes to bf16 ---------------------------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
-// The raw bf16 pattern of a code stands for raw = value * 2^-offset in units of the block scale, so a block's factor is
-// 2^(scale - 127 + offset), in bf16 the exponent field scale + offset.  That field is out of [1, 254] for MXFP blocks with
-// a scale far above one and for MXINT blocks at either end: those tiles take a second factor (kRare).
-template <int kFormat>
-__device__ __forceinline__ int raw_offset(int bits) {
-  if constexpr (kFormat == MXQ_CACHE_INT8)
-    return 1 - bits;
-  else if constexpr (kFormat == MXQ_CACHE_BF16)
-    return 0;
-  else
-    return 127 - ((1 << (Format<kFormat>::E - 1)) - 1);
-}
-template <int kFormat>
-__device__ __forceinline__ bool rare_scale(uint32_t scale, int offset) {
-  if constexpr (kFormat == MXQ_CACHE_INT8)
-    return (int)scale + offset < 1 || scale == 255u;
-  else
-    return (int)scale + offset > 254;
-}
-// first factor of a rare block (bf16 pattern): the field clamped to 254; for MXINT also subnormal powers, and infinity
-// for scale byte 255 (the reference multiplies the zero mantissas of such a block by 2^128)
-template <int kFormat>
-__device__ __forceinline__ uint32_t rare_factor(uint32_t scale, int offset) {
-  const int field = (int)scale + offset;
-  if constexpr (kFormat == MXQ_CACHE_INT8) {
-    if (scale == 255u) return 0x7F80u;
-    return field >= 1 ? (uint32_t)field << 7 : (field > -7 ? 1u << (field + 6) : 0u);
-  }
-  return (uint32_t)min(field, 254) << 7;
-}
-template <int kFormat>
-__device__ __forceinline__ uint32_t rare_rest(uint32_t scale, int offset) {
-  return (uint32_t)(127 + max((int)scale + offset - 254, 0)) << 7;
-}
-
-template <bool kRare>
-__device__ __forceinline__ uint32_t scaled(uint32_t raw, uint32_t f, uint32_t rest) {
-  raw = mul2(raw, f);
-  return kRare ? mul2(raw, rest) : raw;
-}
-
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {  // one instruction
-  uint32_t d;
-  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "r"(mask), "r"(bits));
-  return d;
-}
-// Four 8-bit codes -> upper and lower bytes of their raw bf16 patterns: sign, then exponent and fraction fields moved down
-// to the bf16 fraction boundary.
-template <int kFormat>
-__device__ __forceinline__ void split_bytes(uint32_t w, uint32_t &hi, uint32_t &lo) {
-  if constexpr (kFormat == MXQ_CACHE_E4M3) {
-    hi = and_or(w, 0x80808080u, (w >> 4) & 0x07070707u), lo = (w << 4) & 0xF0F0F0F0u;
-  } else {
-    hi = and_or(w, 0x80808080u, (w >> 3) & 0x0F0F0F0Fu), lo = (w << 5) & 0xE0E0E0E0u;
-  }
-}
-// Eight E2M1 codes -> the same bytes of the even (0, 2, 4, 6) and odd (1, 3, 5, 7) ones.
-__device__ __forceinline__ void split_nibbles(uint32_t w, uint32_t &hi_even, uint32_t &lo_even, uint32_t &hi_odd,
-                                              uint32_t &lo_odd) {
-  hi_even = and_or(w << 4, 0x80808080u, (w >> 2) & 0x01010101u), lo_even = (w << 6) & 0xC0C0C0C0u;
-  hi_odd = and_or(w, 0x80808080u, (w >> 6) & 0x01010101u), lo_odd = (w << 2) & 0xC0C0C0C0u;
-}
-// Two int8, one in the lower byte of each half -> bf16 pair: 128 + (u & 127) minus 128 or 256 by the sign bit.
-__device__ __forceinline__ uint32_t int8_lower(uint32_t x) {
-  return sub2(and_or(x, 0x007F007Fu, 0x43004300u), and_or(x, 0x00800080u, 0x43004300u));
-}
-
-// One word of a key row -> bf16 pairs.  Halves of pair i of the word are these elements, from the word's first one:
-//   16 bit: 0, 1;  E4M3 / E5M2: 2 i, 2 i + 1;  int8: i, i + 2;  E2M1: 4 (i & 1) + (i >> 1) and that + 2
-template <int kFormat>
-__device__ __forceinline__ int pair_element(int i, int half) {
-  if (kFormat == MXQ_CACHE_INT8) return i + 2 * half;
-  if (kFormat == MXQ_CACHE_E2M1X2) return 4 * (i & 1) + (i >> 1) + 2 * half;
-  return 2 * i + half;
-}
-template <int kFormat, bool kRare>
-__device__ __forceinline__ void key_word(uint32_t w, uint32_t f, uint32_t rest, uint32_t *out) {
-  if constexpr (kFormat == MXQ_CACHE_BF16) {
-    out[0] = w;
-  } else if constexpr (kFormat == MXQ_CACHE_INT8) {
-    out[0] = scaled<kRare>(int8_lower(w), f, rest), out[1] = scaled<kRare>(int8_lower(w >> 8), f, rest);
-  } else if constexpr (Format<kFormat>::kBits == 8) {
-    uint32_t hi, lo;
-    split_bytes<kFormat>(w, hi, lo);
-    out[0] = scaled<kRare>(__byte_perm(lo, hi, 0x5140), f, rest), out[1] = scaled<kRare>(__byte_perm(lo, hi, 0x7362), f, rest);
-  } else {
-    uint32_t he, le, ho, lo;
-    split_nibbles(w, he, le, ho, lo);
-    out[0] = scaled<kRare>(__byte_perm(le, he, 0x5140), f, rest), out[1] = scaled<kRare>(__byte_perm(le, he, 0x7362), f, rest);
-    out[2] = scaled<kRare>(__byte_perm(lo, ho, 0x5140), f, rest), out[3] = scaled<kRare>(__byte_perm(lo, ho, 0x7362), f, rest);
-  }
-}
-// The same word of two value rows -> pairs (row a, row b) of its elements 0, 1, 2, ...
-template <int kFormat, bool kRare>
-__device__ __forceinline__ void value_words(uint32_t a, uint32_t b, uint32_t f, uint32_t rest, uint32_t *out) {
-  if constexpr (kFormat == MXQ_CACHE_BF16) {
-    out[0] = __byte_perm(a, b, 0x5410), out[1] = __byte_perm(a, b, 0x7632);
-  } else if constexpr (kFormat == MXQ_CACHE_INT8) {
-    out[0] = scaled<kRare>(int8_lower(__byte_perm(a, b, 0x4400)), f, rest);
-    out[1] = scaled<kRare>(int8_lower(__byte_perm(a, b, 0x5511)), f, rest);
-    out[2] = scaled<kRare>(int8_lower(__byte_perm(a, b, 0x6622)), f, rest);
-    out[3] = scaled<kRare>(int8_lower(__byte_perm(a, b, 0x7733)), f, rest);
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t x = __byte_perm(a, b, h ? 0x7362 : 0x5140);  // bytes a, b, a, b of neighbouring positions
-      if constexpr (Format<kFormat>::kBits == 8) {
-        uint32_t hi, lo;
-        split_bytes<kFormat>(x, hi, lo);
-        out[2 * h] = scaled<kRare>(__byte_perm(lo, hi, 0x5140), f, rest);
-        out[2 * h + 1] = scaled<kRare>(__byte_perm(lo, hi, 0x7362), f, rest);
-      } else {
-        uint32_t he, le, ho, lo;
-        split_nibbles(x, he, le, ho, lo);
-        out[4 * h] = scaled<kRare>(__byte_perm(le, he, 0x5140), f, rest);
-        out[4 * h + 1] = scaled<kRare>(__byte_perm(lo, ho, 0x5140), f, rest);
-        out[4 * h + 2] = scaled<kRare>(__byte_perm(le, he, 0x7362), f, rest);
-        out[4 * h + 3] = scaled<kRare>(__byte_perm(lo, ho, 0x7362), f, rest);
-      }
-    }
-  }
-}
-
 __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -531,8 +397,8 @@ struct Split {
   }
   __device__ __forceinline__ int64_t start(int64_t i) const { return i * q + min(i, r); }
   __device__ __forceinline__ int64_t cta_of(int64_t u) const {  // the CTA that takes unit u
-    const int64_t longer = r * (q + 1);
-    return u < longer ? u / (q + 1) : r + (u - longer) / q;
+    const int64_t longer = r * (q + 1), n = u < longer ? u : u - longer, d = u < longer ? q + 1 : q;
+    return (u < longer ? 0 : r) + (n <= UINT32_MAX && d <= UINT32_MAX ? (uint32_t)n / (uint32_t)d : n / d);
   }
 };
 __device__ __forceinline__ int length_of(const AttnArgs &a, int b) { return clamp_length(a.lengths[b], a.most, a.status); }
@@ -616,6 +482,7 @@ attention_kernel(const Cache c, const Table table, const AttnArgs a) {
   const int t = lane & 3, r = lane >> 2;
   uint8_t *ring = smem + warp * (S::kStages * S::kStage);
 
+  wait_for_previous();
   const int rows = c.heads * a.head_tiles;
   const int64_t total = units_between(a, 0, a.batch, lane) * rows;
   const int64_t ctas = min((int64_t)a.ctas, total);
@@ -775,7 +642,7 @@ attention_kernel(const Cache c, const Table table, const AttnArgs a) {
         w.template tile<false>(st, live, c.bits, a, ((int64_t)here.b * rows + here.row) * a.score_tokens + tok, lane);
     }
     stage = stage == S::kStages - 1 ? 0 : stage + 1;
-    if (i + 1 == todo) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (i + 1 == todo) let_next_start();
     if (here.unit + 1 < work && i + 1 < todo) {
       ++here.unit;
       continue;
@@ -846,86 +713,100 @@ attention_kernel(const Cache c, const Table table, const AttnArgs a) {
 // Joins the parts of the rows that CTAs share, and adds the softmax weights of every token to the caller's statistics:
 //   weights[b, head, j] += sum over the group of exp(s_j - m) / l.
 // grid: (x, heads, batch): heads g of a group with g % x == blockIdx.x are joined by the CTA, tokens are strided over x.
+// Before the wait only what the attention kernel does not write is read: its CTAs let this kernel start after their own
+// wait, so everything before it in the stream has finished.
 template <typename T>
 __global__ void __launch_bounds__(kFinishThreads)
 finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
-  extern __shared__ float sm[];  // [4][dim] sums of the warps, then [group] pairs of maximum and 1 / sum
-  float2 *stats = reinterpret_cast<float2 *>(sm + 4 * dim);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  extern __shared__ float4 sm[];  // [kFinishThreads], then [group] pairs of maximum and 1 / sum
+  float2 *stats = reinterpret_cast<float2 *>(sm + kFinishThreads);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int head = blockIdx.y, b = blockIdx.z;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int rows = heads * a.head_tiles;
   const int64_t before = units_between(a, 0, b, lane);
-  const int n = units_of_length(length_of(a, b));
-  const int64_t total = (before + units_between(a, b, a.batch, lane)) * rows;
+  const int length = length_of(a, b), n = units_of_length(length);
+  const int64_t total = (before + n + units_between(a, b + 1, a.batch, lane)) * rows;
   const Split split(total, min((int64_t)a.ctas, total));
 
   // CTAs first .. last hold the parts of head g's row; part of CTA c in its slot 0 or 1
-  auto locate = [&](int g, int64_t &first, int64_t &last, bool &late) {
+  auto locate = [&](int g, int &first, int &last, bool &late) {
     const int64_t u0 = before * rows + (int64_t)(head * a.head_tiles + g / tile_heads) * n;
-    first = split.cta_of(u0), last = split.cta_of(u0 + n - kRowCost - 1);
+    first = (int)split.cta_of(u0), last = (int)split.cta_of(u0 + n - kRowCost - 1);
     late = split.start(first) < u0;  // the row is not the first one of its first CTA
   };
-  auto part_of = [&](int64_t c, int64_t first, bool late, int g) {
-    return (c * 2 + (c == first && late ? 1 : 0)) * tile_heads + g % tile_heads;
+  auto part_of = [&](int c, int first, bool late, int g) {
+    return (int64_t)(c * 2 + (c == first && late ? 1 : 0)) * tile_heads + g % tile_heads;
   };
   // maximum and sum of head g, by a whole warp
-  auto join = [&](int g) {
-    int64_t first, last;
-    bool late;
-    locate(g, first, last, late);
+  auto join = [&](int g, int first, int last, bool late) {
     if (first == last) return a.stats != nullptr ? a.stats[(int64_t)b * a.q_heads + head * a.group + g] : make_float2(0.f, 0.f);
-    float top = kLowest;
-    for (int64_t c = first + lane; c <= last; c += 32) top = fmaxf(top, a.part_ml[part_of(c, first, late, g)].x);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, x));
-    float sum = 0.f;
-    for (int64_t c = first + lane; c <= last; c += 32) {
+    float top = kLowest, sum = 0.f;
+    for (int c = first + lane; c <= last; c += 32) {  // running maximum and sum: one pass over the parts
       const float2 p = a.part_ml[part_of(c, first, late, g)];
-      sum += p.y * exp2f(p.x - top);
+      const float high = fmaxf(top, p.x);
+      sum = sum * exp2f(top - high) + p.y * exp2f(p.x - high), top = high;
     }
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+    for (int x = 16; x > 0; x >>= 1) {
+      const float t2 = __shfl_xor_sync(0xFFFFFFFFu, top, x), s2 = __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+      const float high = fmaxf(top, t2);
+      sum = sum * exp2f(top - high) + s2 * exp2f(t2 - high), top = high;
+    }
     return make_float2(top, sum);
   };
+  int first, last;
+  bool late;
+  locate(blockIdx.x, first, last, late);
+  wait_for_previous();
 
+  const int vecs = dim >> 2, groups = kFinishThreads / vecs, vec = tid & (vecs - 1), group = tid / vecs;
   for (int g = blockIdx.x; g < a.group; g += gridDim.x) {
-    int64_t first, last;
-    bool late;
-    locate(g, first, last, late);
+    if (g != blockIdx.x) locate(g, first, last, late);
     if (first == last) continue;  // finished by its CTA
-    const float2 st = join(g);
-    for (int d0 = 0; d0 < dim; d0 += 32) {
-      float v = 0.f;
-      for (int64_t c = first + warp; c <= last; c += 4) {
-        const int64_t part = part_of(c, first, late, g);
-        v += exp2f(a.part_ml[part].x - st.x) * a.part_o[part * dim + d0 + lane];
-      }
-      sm[warp * dim + d0 + lane] = v;
+    const float2 st = join(g, first, last, late);
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = first + group; c <= last; c += groups) {
+      const int64_t part = part_of(c, first, late, g);
+      const float f = exp2f(a.part_ml[part].x - st.x);
+      const float4 o = reinterpret_cast<const float4 *>(a.part_o + part * dim)[vec];
+      v.x += f * o.x, v.y += f * o.y, v.z += f * o.z, v.w += f * o.w;
     }
+    sm[tid] = v;
     __syncthreads();
-    for (int d = threadIdx.x; d < dim; d += kFinishThreads) {
-      const float v = sm[d] + sm[dim + d] + sm[2 * dim + d] + sm[3 * dim + d];
-      store_scalar(static_cast<T *>(a.out) + ((int64_t)b * a.q_heads + head * a.group + g) * dim + d,
-                   st.y == 0.f ? 0.f : v / st.y);
+    if (tid < vecs) {
+      for (int k = 1; k < groups; ++k) {
+        const float4 o = sm[k * vecs + tid];
+        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+      }
+      const float f = st.y == 0.f ? 0.f : 1.f;
+      T *out = static_cast<T *>(a.out) + ((int64_t)b * a.q_heads + head * a.group + g) * dim + 4 * tid;
+      const float r[4] = {f == 0.f ? 0.f : v.x / st.y, f == 0.f ? 0.f : v.y / st.y, f == 0.f ? 0.f : v.z / st.y,
+                          f == 0.f ? 0.f : v.w / st.y};
+      store_vals(out, 0, r);
     }
     __syncthreads();
   }
   if (a.weights == nullptr) return;
   for (int g = warp; g < a.group; g += kFinishThreads / 32) {
-    const float2 st = join(g);
+    locate(g, first, last, late);
+    const float2 st = join(g, first, last, late);
     if (lane == 0) stats[g] = make_float2(st.x, st.y == 0.f ? 0.f : 1.f / st.y);
   }
   __syncthreads();
-  const int length = length_of(a, b);
-  for (int j = blockIdx.x * kFinishThreads + threadIdx.x; j < length; j += gridDim.x * kFinishThreads) {
+  const float *scores = a.scores + ((int64_t)b * rows + head * a.head_tiles) * a.score_tokens * tile_heads;
+  float *weights = a.weights + ((int64_t)b * heads + head) * a.weights_width;
+  for (int j = blockIdx.x * kFinishThreads + tid; j < length; j += gridDim.x * kFinishThreads) {
     float sum = 0.f;
-    for (int g = 0; g < a.group; ++g) {
-      const int64_t row = (int64_t)b * rows + head * a.head_tiles + g / tile_heads;
-      const float s = a.scores[(row * a.score_tokens + j) * tile_heads + g % tile_heads];
-      sum += exp2f(s - stats[g].x) * stats[g].y;
+    for (int g0 = 0; g0 < a.group; g0 += 4) {  // four heads of a tile lie together
+      const int ht = g0 / tile_heads;
+      const float4 s = *reinterpret_cast<const float4 *>(scores + ((int64_t)ht * a.score_tokens + j) * tile_heads + (g0 - ht * tile_heads));
+      sum += exp2f(s.x - stats[g0].x) * stats[g0].y;
+      if (g0 + 1 < a.group) sum += exp2f(s.y - stats[g0 + 1].x) * stats[g0 + 1].y;
+      if (g0 + 2 < a.group) sum += exp2f(s.z - stats[g0 + 2].x) * stats[g0 + 2].y;
+      if (g0 + 3 < a.group) sum += exp2f(s.w - stats[g0 + 3].x) * stats[g0 + 3].y;
     }
-    a.weights[((int64_t)b * heads + head) * a.weights_width + j] += sum;
+    weights[j] += sum;
   }
 }
 
@@ -976,8 +857,7 @@ static int launch_one(const Cache &c, const Table &t, AttnArgs &a, int64_t most_
   int64_t ctas = (int64_t)gemm::sm_count() * (per_sm < kMostPerSm ? per_sm : kMostPerSm);
   if (ctas > most_ctas) ctas = most_ctas;
   a.ctas = (int)ctas;
-  kernel<<<(unsigned)ctas, kWarps * 32, kSmem, st>>>(c, t, a);
-  return cudaGetLastError() == cudaSuccess ? MXQ_OK : MXQ_ERR_LAUNCH;
+  return launch_chained(kernel, dim3((unsigned)ctas), kWarps * 32, kSmem, st, c, t, a);
 }
 template <typename T, int kFormat, int D>
 static int launch_dim(const Cache &c, const Table &t, AttnArgs &a, int nt, int64_t most_ctas, cudaStream_t st) {
@@ -999,23 +879,6 @@ static int launch_attention(int format, int dim, const Cache &c, const Table &t,
   MXQ_PAGED_FORMATS(CALL)
 #undef CALL
   return MXQ_ERR_FORMAT;
-}
-
-// The finish kernel is launched while the attention kernel drains and waits on the device for its end.
-template <typename T>
-static int launch_finish(const AttnArgs &a, int heads, int tile_heads, int dim, unsigned x, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(x, (unsigned)heads, (unsigned)a.batch), cfg.blockDim = dim3(kFinishThreads);
-  cfg.dynamicSmemBytes = 4 * dim * 4 + (a.weights != nullptr ? a.group * sizeof(float2) : 0), cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr, cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, finish_kernel<T>, a, heads, tile_heads, dim) != cudaSuccess) {
-    cudaGetLastError();
-    return MXQ_ERR_LAUNCH;
-  }
-  return MXQ_OK;
 }
 
 }  // namespace paged
@@ -1067,6 +930,7 @@ int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, 
   int64_t group;
   if ((rc = check_attention(cache, batch, q_heads, table_width, c.page_log2, group)) != MXQ_OK) return rc;
   if (!q || !out || !lengths) return MXQ_ERR_NULL;
+  if (!aligned(out, 16)) return MXQ_ERR_ALIGN;
   if (weights && weights_width < 1) return MXQ_ERR_SHAPE;
   const int dim = cache->head_dim;
   const int64_t tokens = table_width << c.page_log2;
@@ -1107,8 +971,11 @@ int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, 
     const int64_t cap = ((int64_t)gemm::sm_count() * 16 + c.heads * batch - 1) / (c.heads * batch);
     x = need < cap ? need : cap;
   }
-  return dtype == MXQ_BF16 ? launch_finish<__nv_bfloat16>(a, c.heads, 8 * nt, dim, (unsigned)x, st)
-                           : launch_finish<float>(a, c.heads, 8 * nt, dim, (unsigned)x, st);
+  const dim3 grid((unsigned)x, (unsigned)c.heads, (unsigned)batch);
+  const size_t smem = kFinishThreads * 16 + (weights ? group * sizeof(float2) : 0);
+  return dtype == MXQ_BF16
+             ? launch_chained(finish_kernel<__nv_bfloat16>, grid, kFinishThreads, smem, st, a, c.heads, 8 * nt, dim)
+             : launch_chained(finish_kernel<float>, grid, kFinishThreads, smem, st, a, c.heads, 8 * nt, dim);
 }
 
 }  // extern "C"

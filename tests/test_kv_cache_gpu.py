@@ -145,6 +145,20 @@ def test_append_then_gather_equals_the_oracle(name, dtype, dim, page, heads):
         assert bool(same[~written].all())
 
 
+@pytest.mark.parametrize("name", ["e4m3", "e5m2", "e2m1", "int8", "int5"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gather_at_the_ends_of_the_range(name, dtype):
+    """Blocks of every magnitude a float has, from subnormal results to the largest finite ones."""
+    n = 250
+    cache, table = make_cache(name, 1, 32, 16, [n])
+    x = rows(1, 1, n, 32, seed=7, dtype=torch.float32, spread=1.0)
+    x = x / x.abs().amax(-1, keepdim=True) * torch.exp2(torch.arange(n).float() - 124)[None, None, :, None]
+    x = x.to(dtype)
+    mb.paged_kv_append(cache, x.to(DEV), x.to(DEV), table, i32([0]))
+    for got in mb.paged_kv_gather(cache, table, i32([n]), n, dtype):
+        assert_bits_equal(got, fake(x, name), name, signed_zero=False)
+
+
 @pytest.mark.parametrize("name", ["e4m3", "e5m2", "int8", "int5"])
 def test_codes_are_those_of_the_plain_quantizers(name):
     cache, table = make_cache(name, 2, 64, 16, [16], spare=0)
