@@ -1,6 +1,7 @@
 // Paged key/value cache in MX formats: writing new rows (mxq_paged_append), reading rows back (mxq_paged_gather) and
 // evicting the tokens with the least accumulated attention weight (mxq_paged_evict).
 
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -297,12 +298,15 @@ gather_kernel(const Cache c, const Table table, const int32_t *lengths, T *key, 
 }
 
 // ---- evict -----------------------------------------------------------------------------------------------------------
-// Selection: one CTA per (sequence, head).  The weights become 32-bit keys whose unsigned order is the order of
-// preference; three passes over 11 + 11 + 10 bits of the keys (a histogram in shared memory each) find the key of the
-// last token kept, and every warp then walks a contiguous part of the slots with ballots, so that ranks follow the slot
-// order.  Keys live in shared memory when they fit and are read again from L2 otherwise.
-constexpr int kSelectThreads = 1024;
+// Selection: a cluster of 1 to 8 CTAs per (sequence, head), each with a contiguous part of the slots.  The weights become
+// 32-bit keys whose unsigned order is the order of preference; three passes over 11 + 11 + 10 bits of the keys (a
+// histogram in each CTA's shared memory, added up over the cluster) find the key of the last token kept, and every warp
+// then walks a contiguous part of the slots, four neighbours a lane, so that ranks follow the slot order.  Keys live in shared memory
+// when they fit and are read again from L2 otherwise.
+constexpr int kSelectThreads = 512;
+constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kBins = 2048;
+constexpr int kSlotsPerCta = 2048;  // rows of more slots are shared by a cluster
 constexpr int kKeysInShared = 48 * 1024;
 
 struct EvictArgs {
@@ -323,32 +327,51 @@ __device__ __forceinline__ uint32_t key_of(float w) {
   return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-// exclusive prefix sum over the CTA's 32 warps of a per-warp value held by every lane; `total` = the sum
+namespace cg = cooperative_groups;
+
+__device__ __forceinline__ int warp_total(int v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, o);
+  return v;
+}
+__device__ __forceinline__ int warp_scan(int v) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int x = __shfl_up_sync(0xFFFFFFFFu, v, o);
+    if ((int)(threadIdx.x & 31) >= o) v += x;
+  }
+  return v;
+}
+// exclusive prefix sum over the CTA's warps of a per-warp value held by every lane; `total` = the sum
 __device__ __forceinline__ int scan_warps(int v, int *scratch, int &total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   __syncthreads();
   if (lane == 0) scratch[warp] = v;
   __syncthreads();
-  int s = scratch[lane];
+  int s = lane < kSelectWarps ? scratch[lane] : 0;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
+  for (int o = 1; o < kSelectWarps; o <<= 1) {
     const int n = __shfl_up_sync(0xFFFFFFFFu, s, o);
     if (lane >= o) s += n;
   }
-  total = __shfl_sync(0xFFFFFFFFu, s, 31);
+  total = __shfl_sync(0xFFFFFFFFu, s, kSelectWarps - 1);
   const int before = __shfl_sync(0xFFFFFFFFu, s, warp == 0 ? 0 : warp - 1);
   return warp == 0 ? 0 : before;
 }
 
+// grid: (heads * cluster, batch)
 __global__ void __launch_bounds__(kSelectThreads)
 evict_select_kernel(const Cache c, int64_t table_tokens, const EvictArgs a) {
+  extern __shared__ __align__(16) uint32_t keys[];
+  __shared__ __align__(16) int hist[3][kBins];  // one per pass: the CTAs of a cluster read each other's without a second barrier
+  __shared__ int scratch[kSelectWarps];
+  __shared__ int found[2];   // bin of the last kept key, keys in bins above it
+  __shared__ int counts[3];  // of this CTA's part: keys equal to the last one, holes, movers
+  cg::cluster_group cluster = cg::this_cluster();
+  const int size = cluster.num_blocks(), rank = cluster.block_rank();
   wait_for_previous();
   let_next_start();
-  extern __shared__ uint32_t keys[];
-  __shared__ int hist[kBins];
-  __shared__ int scratch[32];
-  __shared__ int found[2];  // bin of the last kept key, keys in bins above it
-  const int head = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int head = blockIdx.x / size, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t b = blockIdx.y;
   const int64_t row = b * c.heads + head;
   const int n = clamp_length(a.lengths[b], min(table_tokens, a.width), a.status);
@@ -357,27 +380,55 @@ evict_select_kernel(const Cache c, int64_t table_tokens, const EvictArgs a) {
   const int32_t *p = a.positions != nullptr ? a.positions + row * a.width : nullptr;
   float *nw = a.new_weights + row * a.width;
   int32_t *np = a.new_positions + row * a.width;
-  if (head == 0 && tid == 0) a.new_lengths[b] = m;
-  for (int64_t j = m + tid; j < a.width; j += kSelectThreads) nw[j] = 0.f, np[j] = -1;
-  if (n <= a.keep) {
-    for (int j = tid; j < n; j += kSelectThreads) nw[j] = w[j], np[j] = p != nullptr ? p[j] : j;
-    if (tid == 0) a.moves[row] = 0;
+  if (head == 0 && rank == 0 && tid == 0) a.new_lengths[b] = m;
+  for (int64_t j = m + rank * kSelectThreads + tid; j < a.width; j += size * kSelectThreads) nw[j] = 0.f, np[j] = -1;
+  // this CTA's part of the slots, whole warps of it each
+  const int begin = (int)min((int64_t)rank * ((n + size - 1) / size), (int64_t)n);
+  const int end = min(begin + (n + size - 1) / size, n);
+  if (n <= a.keep) {  // the same for every CTA of the cluster
+    for (int j = begin + tid; j < end; j += kSelectThreads) nw[j] = w[j], np[j] = p != nullptr ? p[j] : j;
+    if (rank == 0 && tid == 0) a.moves[row] = 0;
     return;
   }
   const int64_t first_safe = (int64_t)(p != nullptr && a.next_position != nullptr ? a.next_position[b] : n) - a.recent;
-  const bool shared_keys = n <= kKeysInShared;
-  auto make_key = [&](int j) {
-    const int64_t pos = p != nullptr ? p[j] : j;
-    return pos >= first_safe ? 0xFFFFFFFFu : key_of(w[j]);
+  const int mine = end - begin;
+  const bool shared_keys = mine <= kKeysInShared;
+  auto make_key = [&](float x, int pos) { return pos >= first_safe ? 0xFFFFFFFFu : key_of(x); };
+  // keys of the four slots from begin + l on (l a multiple of 4); what lies behind the part is not used
+  auto load4 = [&](int l, uint32_t (&k)[4]) {
+    if (shared_keys) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(keys + l);
+      k[0] = v.x, k[1] = v.y, k[2] = v.z, k[3] = v.w;
+    } else {
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int j = min(begin + l + x, end - 1);
+        k[x] = make_key(w[j], p != nullptr ? p[j] : j);
+      }
+    }
   };
-  auto key_at = [&](int j) { return shared_keys ? keys[j] : make_key(j); };
+  for (int k = tid; k < 3 * kBins; k += kSelectThreads) (&hist[0][0])[k] = 0;
+  __syncthreads();
   // every slot below `keep` starts out with its own statistics; the move kernel overwrites those that are filled anew
-#pragma unroll 8
-  for (int j = tid; j < n; j += kSelectThreads) {
-    const float x = w[j];
-    const int pos = p != nullptr ? p[j] : j;
-    if (j < m) nw[j] = x, np[j] = pos;
-    if (shared_keys) keys[j] = pos >= first_safe ? 0xFFFFFFFFu : key_of(x);
+  constexpr int kBatch = 8;  // reads in flight
+  for (int j0 = begin + tid; j0 < end; j0 += kSelectThreads * kBatch) {
+    float x[kBatch];
+    int pos[kBatch];
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int j = j0 + k * kSelectThreads;
+      x[k] = j < end ? w[j] : 0.f, pos[k] = j < end && p != nullptr ? p[j] : j;
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int j = j0 + k * kSelectThreads;
+      if (j < end) {
+        if (j < m) nw[j] = x[k], np[j] = pos[k];
+        const uint32_t key = make_key(x[k], pos[k]);
+        if (shared_keys) keys[j - begin] = key;
+        atomicAdd(&hist[0][key >> 21], 1);
+      }
+    }
   }
 
   uint32_t prefix = 0;  // the digits found so far, in place
@@ -386,78 +437,133 @@ evict_select_kernel(const Cache c, int64_t table_tokens, const EvictArgs a) {
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
     const int bins = pass == 2 ? 1024 : 2048;
-    const uint32_t above = pass == 0 ? 0u : (pass == 1 ? 0xFFE00000u : 0xFFFFFC00u);
+    const uint32_t above = pass == 1 ? 0xFFE00000u : 0xFFFFFC00u;
     __syncthreads();
-    for (int k = tid; k < kBins; k += kSelectThreads) hist[k] = 0;
-    __syncthreads();
-    for (int j = tid; j < n; j += kSelectThreads) {
-      const uint32_t k = key_at(j);
-      if ((k & above) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+    if (pass > 0) {
+      for (int l = 4 * tid; l < mine; l += 4 * kSelectThreads) {
+        uint32_t k[4];
+        load4(l, k);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if ((k[x] & above) == prefix && l + x < mine) atomicAdd(&hist[pass][(k[x] >> shift) & (bins - 1)], 1);
+      }
     }
-    __syncthreads();
-    // thread t owns bins bins - 1 - 2t and bins - 2 - 2t: the running sum goes from the largest key down
-    const int hi = bins - 1 - 2 * tid, lo = hi - 1;
-    const int ch = hi >= 0 ? hist[hi] : 0, cl = lo >= 0 ? hist[lo] : 0;
-    int s = ch + cl;
+    if (size > 1)
+      cluster.sync();
+    else
+      __syncthreads();
+    // thread t owns kOwn bins from bins - 1 - kOwn * t down: the running sum goes from the largest key down
+    constexpr int kOwn = kBins / kSelectThreads;
+    static_assert(kOwn == 4, "a thread reads its bins as one vector");
+    int cnt[kOwn] = {}, s = 0;
+    const int low = bins - kOwn - kOwn * tid;
+    if (low >= 0)
+      for (int r = 0; r < size; ++r) {
+        const int4 h = *reinterpret_cast<const int4 *>(size > 1 ? cluster.map_shared_rank(&hist[pass][low], r) : &hist[pass][low]);
+        cnt[0] += h.w, cnt[1] += h.z, cnt[2] += h.y, cnt[3] += h.x;
+      }
+    s = cnt[0] + cnt[1] + cnt[2] + cnt[3];
+    int run = s;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xFFFFFFFFu, s, o);
-      if (lane >= o) s += x;
+      const int x = __shfl_up_sync(0xFFFFFFFFu, run, o);
+      if (lane >= o) run += x;
     }
     int total;
-    const int base = scan_warps(__shfl_sync(0xFFFFFFFFu, s, 31), scratch, total) + s - ch - cl;
-    if (base < need && base + ch >= need) found[0] = hi, found[1] = base;
-    if (base + ch < need && base + ch + cl >= need) found[0] = lo, found[1] = base + ch;
+    int base = scan_warps(__shfl_sync(0xFFFFFFFFu, run, 31), scratch, total) + run - s;
+#pragma unroll
+    for (int x = 0; x < kOwn; ++x) {
+      if (base < need && base + cnt[x] >= need) found[0] = low + kOwn - 1 - x, found[1] = base;
+      base += cnt[x];
+    }
     __syncthreads();
     prefix |= (uint32_t)found[0] << shift;
     need -= found[1];
   }
   const uint32_t last = prefix;  // tokens above it are kept, and the first `need` equal to it
 
-  const int part = ((n + 1023) / 1024) * 32;  // slots of one warp
-  const int begin = min(warp * part, n), end = min(begin + part, n);
-  int ties = 0, total;
-  for (int j0 = begin; j0 < end; j0 += 32)
-    ties += __popc(__ballot_sync(0xFFFFFFFFu, j0 + lane < end && key_at(min(j0 + lane, n - 1)) == last));
-  const int ties_before = scan_warps(ties, scratch, total);
-  const uint32_t below = (1u << lane) - 1u;
-  int holes = 0, movers = 0, seen = ties_before;
-  auto classify = [&](int j, bool in, bool &kept) {
-    const uint32_t k = in ? key_at(j) : 0u;
-    const uint32_t tie = __ballot_sync(0xFFFFFFFFu, in && k == last);
-    kept = in && (k > last || (k == last && seen + __popc(tie & below) < need));
-    seen += __popc(tie);
+  // Count, for every warp's part of the slots: keys above the last one and equal to it, below and from `keep` on.
+  const int part = (mine + kSelectWarps * 128 - 1) / (kSelectWarps * 128) * 128;
+  const int first = min(warp * part, mine), stop = min(first + part, mine);
+  const int edge = max(0, min(m - begin, mine));  // slots of this CTA before it lie below `keep`
+  int more_low = 0, more_high = 0, tie_low = 0, tie_high = 0;
+  for (int l = first + 4 * lane; l < stop; l += 128) {
+    uint32_t k[4];
+    load4(l, k);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const bool in = l + x < stop, low = l + x < edge;
+      more_low += in && low && k[x] > last, more_high += in && !low && k[x] > last;
+      tie_low += in && low && k[x] == last, tie_high += in && !low && k[x] == last;
+    }
+  }
+  more_low = warp_total(more_low), more_high = warp_total(more_high);
+  tie_low = warp_total(tie_low), tie_high = warp_total(tie_high);
+  // sum over the CTAs before this one of one of their counts
+  auto before = [&](int which) {
+    int sum = 0;
+    for (int r = 0; r < rank; ++r) sum += *cluster.map_shared_rank(&counts[which], r);
+    return sum;
   };
-  for (int j0 = begin; j0 < end; j0 += 32) {
-    const int j = j0 + lane;
-    bool kept;
-    classify(j, j < end, kept);
-    holes += __popc(__ballot_sync(0xFFFFFFFFu, j < end && j < m && !kept));
-    movers += __popc(__ballot_sync(0xFFFFFFFFu, kept && j >= m));
+  int total;
+  int seen = scan_warps(tie_low + tie_high, scratch, total);  // ties before the warp's part
+  if (size > 1) {
+    if (tid == 0) counts[0] = total;
+    cluster.sync();
+    seen += before(0);
   }
-  int n_moves;
-  int hole_at = scan_warps(holes, scratch, n_moves);
-  int mover_at = scan_warps(movers, scratch, n_moves);
+  const int kept_ties = max(0, min(need - seen, tie_low + tie_high)), kept_low = min(kept_ties, tie_low);
+  const int n_low = max(0, min(edge, stop) - first);
+  int n_holes, n_movers;
+  int hole_at = scan_warps(n_low - more_low - kept_low, scratch, n_holes);
+  int mover_at = scan_warps(more_high + kept_ties - kept_low, scratch, n_movers);
+  if (size > 1) {
+    if (tid == 0) counts[1] = n_holes, counts[2] = n_movers;
+    cluster.sync();
+    hole_at += before(1), mover_at += before(2);
+    if (rank == size - 1 && tid == 0) a.moves[row] = before(1) + n_holes;
+  } else if (tid == 0) {
+    a.moves[row] = n_holes;
+  }
   int32_t *from = a.from + row * a.max_moves, *to = a.to + row * a.max_moves;
-  seen = ties_before;
-  for (int j0 = begin; j0 < end; j0 += 32) {
-    const int j = j0 + lane;
-    bool kept;
-    classify(j, j < end, kept);
-    const bool hole = j < end && j < m && !kept, mover = kept && j >= m;
-    const uint32_t hb = __ballot_sync(0xFFFFFFFFu, hole), mb = __ballot_sync(0xFFFFFFFFu, mover);
-    if (hole) to[hole_at + __popc(hb & below)] = j;
-    if (mover) from[mover_at + __popc(mb & below)] = j;
-    hole_at += __popc(hb), mover_at += __popc(mb);
+  for (int l0 = first; l0 < stop; l0 += 128) {  // the warp takes 128 slots at a time, four neighbours a lane
+    const int l = l0 + 4 * lane;
+    uint32_t k[4] = {};
+    if (l < stop) load4(l, k);
+    int ties = 0;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) ties += l + x < stop && k[x] == last;
+    int rank_of_tie = seen;
+    if (__any_sync(0xFFFFFFFFu, ties != 0)) {
+      const int upto = warp_scan(ties);
+      rank_of_tie += upto - ties, seen += __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    uint32_t holes = 0, movers = 0;  // bit x: slot l + x
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const bool in = l + x < stop, tie = in && k[x] == last;
+      const bool kept = in && (k[x] > last || (tie && rank_of_tie < need));
+      rank_of_tie += tie;
+      holes |= (uint32_t)(in && !kept && l + x < edge) << x, movers |= (uint32_t)(kept && l + x >= edge) << x;
+    }
+    const int both = __popc(holes) | __popc(movers) << 16;
+    const int upto = warp_scan(both), all = __shfl_sync(0xFFFFFFFFu, upto, 31);
+    int h = hole_at + ((upto - both) & 0xFFFF), v = mover_at + ((upto - both) >> 16);
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if ((holes >> x) & 1u) to[h++] = begin + l + x;
+      if ((movers >> x) & 1u) from[v++] = begin + l + x;
+    }
+    hole_at += all & 0xFFFF, mover_at += all >> 16;
   }
-  if (tid == 0) a.moves[row] = n_moves;
+  if (size > 1) cluster.sync();  // no CTA leaves while another may still read its counts
 }
 
-// A warp takes 32 moves at a time: each lane looks one of them up (slots, pages) and moves its statistics, then the warp
+// A warp takes `per_warp` moves at a time (up to 32): each lane looks one of them up (slots, pages) and moves its statistics, then the warp
 // copies the key and value rows of all of them, 16 bytes a lane with four copies in flight.  Sources lie at or above
 // `keep`, destinations below it, so moves never overlap.
 __global__ void __launch_bounds__(kThreads)
-evict_move_kernel(const Cache c, const Table table, const EvictArgs a, int row_bytes_log2, int scale_bytes) {
+evict_move_kernel(const Cache c, const Table table, const EvictArgs a, int row_bytes_log2, int scale_bytes, int per_warp) {
   wait_for_previous();
   let_next_start();
   const int head = blockIdx.y, lane = threadIdx.x & 31;
@@ -467,10 +573,10 @@ evict_move_kernel(const Cache c, const Table table, const EvictArgs a, int row_b
   const int in_page = (1 << c.page_log2) - 1;
   const int32_t *from = a.from + row * a.max_moves, *to = a.to + row * a.max_moves;
   const int pieces_log2 = row_bytes_log2 - 4, pieces = 1 << pieces_log2;  // of 16 bytes
-  const int warps = gridDim.x * (kThreads / 32);
-  for (int i0 = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * 32; i0 < n; i0 += warps * 32) {
+  const int stride = gridDim.x * (kThreads / 32) * per_warp;
+  for (int i0 = (blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5)) * per_warp; i0 < n; i0 += stride) {
     int64_t sr = -1, dr = -1;
-    if (i0 + lane < n) {
+    if (lane < per_warp && i0 + lane < n) {
       const int s = from[i0 + lane], d = to[i0 + lane];
       a.new_weights[row * a.width + d] = a.weights[row * a.width + s];
       a.new_positions[row * a.width + d] = a.positions != nullptr ? a.positions[row * a.width + s] : s;
@@ -480,7 +586,7 @@ evict_move_kernel(const Cache c, const Table table, const EvictArgs a, int row_b
       else
         sr += s & in_page, dr += d & in_page;
     }
-    const int live = min(n - i0, 32);
+    const int live = min(n - i0, per_warp);
     // 16-byte pieces of the moves in order: [move][side][piece]
     const int total = live << (pieces_log2 + 1);
     for (int k0 = 0; k0 < total; k0 += 128) {
@@ -563,8 +669,8 @@ int mxq_paged_append(const mxq_paged_cache *cache, const void *key, const void *
 #define CALL(f)                                                                                                            \
   if (cache->format == f)                                                                                                  \
     return dtype == MXQ_BF16                                                                                               \
-               ? launch_chained(append_kernel<__nv_bfloat16, f>, grid, kThreads, 0, st, c, t, a, log2_of(dim), tab)        \
-               : launch_chained(append_kernel<float, f>, grid, kThreads, 0, st, c, t, a, log2_of(dim), tab);
+               ? launch_chained(append_kernel<__nv_bfloat16, f>, grid, kThreads, 0, st, 1, c, t, a, log2_of(dim), tab)        \
+               : launch_chained(append_kernel<float, f>, grid, kThreads, 0, st, 1, c, t, a, log2_of(dim), tab);
   MXQ_PAGED_FORMATS(CALL)
 #undef CALL
   return MXQ_ERR_FORMAT;
@@ -589,9 +695,9 @@ int mxq_paged_gather(const mxq_paged_cache *cache, void *key, void *value, int d
   cudaStream_t st = (cudaStream_t)stream;
 #define CALL(f)                                                                                                             \
   if (cache->format == f)                                                                                                   \
-    return dtype == MXQ_BF16 ? launch_chained(gather_kernel<__nv_bfloat16, f>, grid, kThreads, 0, st, c, t, lengths,        \
+    return dtype == MXQ_BF16 ? launch_chained(gather_kernel<__nv_bfloat16, f>, grid, kThreads, 0, st, 1, c, t, lengths,        \
                                               (__nv_bfloat16 *)key, (__nv_bfloat16 *)value, max_tokens, log2_of(dim), status) \
-                             : launch_chained(gather_kernel<float, f>, grid, kThreads, 0, st, c, t, lengths, (float *)key,  \
+                             : launch_chained(gather_kernel<float, f>, grid, kThreads, 0, st, 1, c, t, lengths, (float *)key,  \
                                               (float *)value, max_tokens, log2_of(dim), status);
   MXQ_PAGED_FORMATS(CALL)
 #undef CALL
@@ -632,7 +738,9 @@ int mxq_paged_evict(const mxq_paged_cache *cache, int64_t batch, const int32_t *
   a.status = status;
   const Table t{page_table, table_stride, table_width};
   cudaStream_t st = (cudaStream_t)stream;
-  const int64_t n_keys = width < kKeysInShared ? width : kKeysInShared;
+  // Clusters of up to 8 CTAs share a row's slots where that leaves no more than two CTAs per SM.
+  int cluster = 1;
+  while (cluster < 8 && width / cluster > kSlotsPerCta && rows * cluster < gemm::sm_count()) cluster *= 2;
   static std::atomic<bool> set_up[64];  // the kernel's shared memory limit has been raised on this device
   int device = 0;
   if (cudaGetDevice(&device) != cudaSuccess) return MXQ_ERR_LAUNCH;
@@ -644,13 +752,19 @@ int mxq_paged_evict(const mxq_paged_cache *cache, int64_t batch, const int32_t *
     }
     set_up[device & 63].store(true, std::memory_order_relaxed);
   }
-  rc = launch_chained(evict_select_kernel, dim3((unsigned)c.heads, (unsigned)batch), kSelectThreads, (size_t)n_keys * 4, st, c,
-                      table_width << c.page_log2, a);
+  const int64_t part = (width + cluster - 1) / cluster;
+  const int64_t n_keys = part < kKeysInShared ? (part + 3) / 4 * 4 : kKeysInShared;
+  rc = launch_chained(evict_select_kernel, dim3((unsigned)(c.heads * cluster), (unsigned)batch), kSelectThreads,
+                      (size_t)n_keys * 4, st, cluster, c, table_width << c.page_log2, a);
   if (rc != MXQ_OK || most == 0) return rc;
   const int row_bytes = row_bytes_of(cache->format, cache->head_dim);
   const int scale_bytes = cache->format == MXQ_CACHE_BF16 ? 0 : cache->head_dim / 32;
-  const dim3 grid(grid_x((most + kThreads - 1) / kThreads, rows, 8), (unsigned)c.heads, (unsigned)batch);
-  return launch_chained(evict_move_kernel, grid, kThreads, 0, st, c, t, a, log2_of(row_bytes), scale_bytes);
+  // moves a warp looks up at once: 32, or fewer so that there is work for four warps on every SM
+  int per_warp = 32;
+  while (per_warp > 4 && rows * most < (int64_t)gemm::sm_count() * 4 * per_warp) per_warp /= 2;
+  const int64_t per_cta = kThreads / 32 * per_warp;
+  const dim3 grid(grid_x((most + per_cta - 1) / per_cta, rows, 8), (unsigned)c.heads, (unsigned)batch);
+  return launch_chained(evict_move_kernel, grid, kThreads, 0, st, 1, c, t, a, log2_of(row_bytes), scale_bytes, per_warp);
 }
 
 }  // extern "C"

@@ -242,13 +242,15 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <typename... P, typename... V>
-static int launch_chained(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, V &&...args) {
+static int launch_chained(void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, int cluster, V &&...args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid, cfg.blockDim = dim3((unsigned)threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr, cfg.numAttrs = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster, attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr, cfg.numAttrs = cluster > 1 ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, kernel, P(args)...) != cudaSuccess) {
     cudaGetLastError();
     return MXQ_ERR_LAUNCH;

@@ -857,7 +857,7 @@ static int launch_one(const Cache &c, const Table &t, AttnArgs &a, int64_t most_
   int64_t ctas = (int64_t)gemm::sm_count() * (per_sm < kMostPerSm ? per_sm : kMostPerSm);
   if (ctas > most_ctas) ctas = most_ctas;
   a.ctas = (int)ctas;
-  return launch_chained(kernel, dim3((unsigned)ctas), kWarps * 32, kSmem, st, c, t, a);
+  return launch_chained(kernel, dim3((unsigned)ctas), kWarps * 32, kSmem, st, 1, c, t, a);
 }
 template <typename T, int kFormat, int D>
 static int launch_dim(const Cache &c, const Table &t, AttnArgs &a, int nt, int64_t most_ctas, cudaStream_t st) {
@@ -974,8 +974,8 @@ int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, 
   const dim3 grid((unsigned)x, (unsigned)c.heads, (unsigned)batch);
   const size_t smem = kFinishThreads * 16 + (weights ? group * sizeof(float2) : 0);
   return dtype == MXQ_BF16
-             ? launch_chained(finish_kernel<__nv_bfloat16>, grid, kFinishThreads, smem, st, a, c.heads, 8 * nt, dim)
-             : launch_chained(finish_kernel<float>, grid, kFinishThreads, smem, st, a, c.heads, 8 * nt, dim);
+             ? launch_chained(finish_kernel<__nv_bfloat16>, grid, kFinishThreads, smem, st, 1, a, c.heads, 8 * nt, dim)
+             : launch_chained(finish_kernel<float>, grid, kFinishThreads, smem, st, 1, a, c.heads, 8 * nt, dim);
 }
 
 }  // extern "C"

@@ -383,18 +383,22 @@ def test_eviction(name, dim, page, keep, recent, positions):
         assert bool((t.view(torch.uint8) == u.view(torch.uint8)).all(-1).all(1).cpu()[free].all())
 
 
-def test_eviction_of_a_row_that_does_not_fit_shared_memory():
-    """More slots than the selection keeps keys of on chip."""
-    n, keep, page = 60000, 20000, 256
-    cache, table = make_cache("none", 1, 32, page, [n], spare=0)
-    x = rows(1, 1, n, 32, seed=81, dtype=torch.bfloat16)
+@pytest.mark.parametrize("heads,n", [(1, 60000), (8, 9000), (150, 50000)])
+def test_eviction_of_long_rows(heads, n):
+    """Rows shared by a cluster of CTAs, and rows of more slots than one CTA keeps keys of on chip."""
+    keep, page = n // 3, 256
+    cache, table = make_cache("none", heads, 32, page, [n], spare=0)
+    x = rows(1, heads, n, 32, seed=81, dtype=torch.bfloat16)
     mb.paged_kv_append(cache, x.to(DEV), x.to(DEV), table, i32([0]))
-    w = torch.rand(1, 1, n, generator=torch.Generator().manual_seed(82)).mul(5000).floor()
+    w = torch.rand(1, heads, n, generator=torch.Generator().manual_seed(82)).mul(5000).floor()
     lens, new_w, pos = mb.paged_kv_evict(cache, table, i32([n]), w.to(DEV), keep, 500)
-    src = plain_evict(w[0, 0].tolist(), list(range(n)), n, n, keep, 500)
-    assert pos[0, 0, :keep].tolist() == src and torch.equal(new_w[0, 0, :keep].cpu(), w[0, 0][src])
     got, _ = mb.paged_kv_gather(cache, table, lens, keep)
-    assert torch.equal(got[0, 0].cpu(), x[0, 0][src])
+    gemm.check_status()
+    for h in {0, heads // 2, heads - 1}:
+        src = plain_evict(w[0, h].tolist(), list(range(n)), n, n, keep, 500)
+        assert pos[0, h, :keep].tolist() == src and torch.equal(new_w[0, h, :keep].cpu(), w[0, h][src])
+        assert torch.equal(got[0, h].cpu(), x[0, h][src])
+    assert bool((pos[..., keep:] == -1).all()) and bool((new_w[..., keep:] == 0).all())
 
 
 # ---- together --------------------------------------------------------------------------------------------------------
