@@ -404,6 +404,8 @@ int mxq_mx_linear_static(const void *x, int in_dtype, const uint8_t *w_codes, co
 #define MXQ_CACHE_E5M2 2
 #define MXQ_CACHE_E2M1X2 3
 #define MXQ_CACHE_INT8 4
+/* largest size of the keys (or values) of one cache that mxq_paged_attention takes: 64 GiB less a row */
+#define MXQ_CACHE_SIDE_BYTES ((int64_t)0xFFFFFFF0 * 16)
 
 typedef struct mxq_paged_cache {
   void *key, *value;

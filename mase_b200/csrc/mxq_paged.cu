@@ -210,22 +210,17 @@ __device__ __forceinline__ void decode16(const uint8_t *p, uint32_t scale, int b
       const uint2 r = __ldcs(reinterpret_cast<const uint2 *>(p));
       key_word<kFormat, kRare>(r.x, f, rest, e), key_word<kFormat, kRare>(r.y, f, rest, e + 4);
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {  // (0, 2) (4, 6) (1, 3) (5, 7) -> (0, 1) (2, 3) (4, 5) (6, 7)
-        out[4 * k] = __byte_perm(e[4 * k], e[4 * k + 2], 0x5410), out[4 * k + 1] = __byte_perm(e[4 * k], e[4 * k + 2], 0x7632);
-        out[4 * k + 2] = __byte_perm(e[4 * k + 1], e[4 * k + 3], 0x5410);
-        out[4 * k + 3] = __byte_perm(e[4 * k + 1], e[4 * k + 3], 0x7632);
+      for (int k = 0; k < 8; k += 4) {  // (0, 4) (1, 5) (2, 6) (3, 7) -> (0, 1) (2, 3) (4, 5) (6, 7)
+        out[k] = __byte_perm(e[k], e[k + 1], 0x5410), out[k + 1] = __byte_perm(e[k + 2], e[k + 3], 0x5410);
+        out[k + 2] = __byte_perm(e[k], e[k + 1], 0x7632), out[k + 3] = __byte_perm(e[k + 2], e[k + 3], 0x7632);
       }
     } else {
       const uint4 r = ld_stream(reinterpret_cast<const uint4 *>(p));
       const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (kFormat == MXQ_CACHE_INT8) {  // (0, 2) (1, 3) -> (0, 1) (2, 3)
-          key_word<kFormat, kRare>(w[k], f, rest, e);
-          out[2 * k] = __byte_perm(e[0], e[1], 0x5410), out[2 * k + 1] = __byte_perm(e[0], e[1], 0x7632);
-        } else {
-          key_word<kFormat, kRare>(w[k], f, rest, &out[2 * k]);
-        }
+      for (int k = 0; k < 4; ++k) {  // (0, 2) (1, 3) -> (0, 1) (2, 3)
+        key_word<kFormat, kRare>(w[k], f, rest, e);
+        out[2 * k] = __byte_perm(e[0], e[1], 0x5410), out[2 * k + 1] = __byte_perm(e[0], e[1], 0x7632);
       }
     }
   }

@@ -158,21 +158,29 @@ __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t b
   asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(d) : "r"(x), "r"(mask), "r"(bits));
   return d;
 }
-// Four 8-bit codes -> upper and lower bytes of their raw bf16 patterns: sign, then exponent and fraction fields moved down
-// to the bf16 fraction boundary.
+// 8-bit codes of bytes 0 and 2 (even) or 1 and 3 (odd) of a word -> raw bf16 pair: the sign to bit 15, exponent and
+// fraction fields down to the bf16 fraction boundary.  Shifts to the left run beside the half-rate logic unit.
 template <int kFormat>
-__device__ __forceinline__ void split_bytes(uint32_t w, uint32_t &hi, uint32_t &lo) {
-  if constexpr (kFormat == MXQ_CACHE_E4M3) {
-    hi = and_or(w, 0x80808080u, (w >> 4) & 0x07070707u), lo = (w << 4) & 0xF0F0F0F0u;
-  } else {
-    hi = and_or(w, 0x80808080u, (w >> 3) & 0x0F0F0F0Fu), lo = (w << 5) & 0xE0E0E0E0u;
-  }
+__device__ __forceinline__ uint32_t raw_even(uint32_t w) {
+  if constexpr (kFormat == MXQ_CACHE_E4M3)
+    return and_or(w << 8, 0x80008000u, (w << 4) & 0x07F007F0u);
+  else
+    return and_or(w << 8, 0x80008000u, (w << 5) & 0x0FE00FE0u);
 }
-// Eight E2M1 codes -> the same bytes of the even (0, 2, 4, 6) and odd (1, 3, 5, 7) ones.
-__device__ __forceinline__ void split_nibbles(uint32_t w, uint32_t &hi_even, uint32_t &lo_even, uint32_t &hi_odd,
-                                              uint32_t &lo_odd) {
-  hi_even = and_or(w << 4, 0x80808080u, (w >> 2) & 0x01010101u), lo_even = (w << 6) & 0xC0C0C0C0u;
-  hi_odd = and_or(w, 0x80808080u, (w >> 6) & 0x01010101u), lo_odd = (w << 2) & 0xC0C0C0C0u;
+template <int kFormat>
+__device__ __forceinline__ uint32_t raw_odd(uint32_t w) {
+  if constexpr (kFormat == MXQ_CACHE_E4M3)
+    return and_or(w, 0x80008000u, (w >> 4) & 0x07F007F0u);
+  else
+    return and_or(w, 0x80008000u, (w >> 3) & 0x0FE00FE0u);
+}
+// E2M1 codes of nibble i of each half -> raw bf16 pair
+template <int i>
+__device__ __forceinline__ uint32_t raw_nibble(uint32_t w) {
+  if constexpr (i == 0) return and_or(w << 12, 0x80008000u, (w << 6) & 0x01C001C0u);
+  if constexpr (i == 1) return and_or(w << 8, 0x80008000u, (w << 2) & 0x01C001C0u);
+  if constexpr (i == 2) return and_or(w << 4, 0x80008000u, (w >> 2) & 0x01C001C0u);
+  return and_or(w, 0x80008000u, (w >> 6) & 0x01C001C0u);
 }
 // Two int8, one in the lower byte of each half -> bf16 pair: 128 + (u & 127) minus 128 or 256 by the sign bit.
 __device__ __forceinline__ uint32_t int8_lower(uint32_t x) {
@@ -180,12 +188,10 @@ __device__ __forceinline__ uint32_t int8_lower(uint32_t x) {
 }
 
 // One word of a key row -> bf16 pairs.  Halves of pair i of the word are these elements, from the word's first one:
-//   16 bit: 0, 1;  E4M3 / E5M2: 2 i, 2 i + 1;  int8: i, i + 2;  E2M1: 4 (i & 1) + (i >> 1) and that + 2
+//   16 bit: 0, 1;  8 bit: i, i + 2;  4 bit: i, i + 4
 template <int kFormat>
 __device__ __forceinline__ int pair_element(int i, int half) {
-  if (kFormat == MXQ_CACHE_INT8) return i + 2 * half;
-  if (kFormat == MXQ_CACHE_E2M1X2) return 4 * (i & 1) + (i >> 1) + 2 * half;
-  return 2 * i + half;
+  return kFormat == MXQ_CACHE_BF16 ? half : i + half * (16 / Format<kFormat>::kBits);
 }
 template <int kFormat, bool kRare>
 __device__ __forceinline__ void key_word(uint32_t w, uint32_t f, uint32_t rest, uint32_t *out) {
@@ -194,45 +200,19 @@ __device__ __forceinline__ void key_word(uint32_t w, uint32_t f, uint32_t rest, 
   } else if constexpr (kFormat == MXQ_CACHE_INT8) {
     out[0] = scaled<kRare>(int8_lower(w), f, rest), out[1] = scaled<kRare>(int8_lower(w >> 8), f, rest);
   } else if constexpr (Format<kFormat>::kBits == 8) {
-    uint32_t hi, lo;
-    split_bytes<kFormat>(w, hi, lo);
-    out[0] = scaled<kRare>(__byte_perm(lo, hi, 0x5140), f, rest), out[1] = scaled<kRare>(__byte_perm(lo, hi, 0x7362), f, rest);
+    out[0] = scaled<kRare>(raw_even<kFormat>(w), f, rest), out[1] = scaled<kRare>(raw_odd<kFormat>(w), f, rest);
   } else {
-    uint32_t he, le, ho, lo;
-    split_nibbles(w, he, le, ho, lo);
-    out[0] = scaled<kRare>(__byte_perm(le, he, 0x5140), f, rest), out[1] = scaled<kRare>(__byte_perm(le, he, 0x7362), f, rest);
-    out[2] = scaled<kRare>(__byte_perm(lo, ho, 0x5140), f, rest), out[3] = scaled<kRare>(__byte_perm(lo, ho, 0x7362), f, rest);
+    out[0] = scaled<kRare>(raw_nibble<0>(w), f, rest), out[1] = scaled<kRare>(raw_nibble<1>(w), f, rest);
+    out[2] = scaled<kRare>(raw_nibble<2>(w), f, rest), out[3] = scaled<kRare>(raw_nibble<3>(w), f, rest);
   }
 }
 // The same word of two value rows -> pairs (row a, row b) of its elements 0, 1, 2, ...
 template <int kFormat, bool kRare>
 __device__ __forceinline__ void value_words(uint32_t a, uint32_t b, uint32_t f, uint32_t rest, uint32_t *out) {
-  if constexpr (kFormat == MXQ_CACHE_BF16) {
-    out[0] = __byte_perm(a, b, 0x5410), out[1] = __byte_perm(a, b, 0x7632);
-  } else if constexpr (kFormat == MXQ_CACHE_INT8) {
-    out[0] = scaled<kRare>(int8_lower(__byte_perm(a, b, 0x4400)), f, rest);
-    out[1] = scaled<kRare>(int8_lower(__byte_perm(a, b, 0x5511)), f, rest);
-    out[2] = scaled<kRare>(int8_lower(__byte_perm(a, b, 0x6622)), f, rest);
-    out[3] = scaled<kRare>(int8_lower(__byte_perm(a, b, 0x7733)), f, rest);
-  } else {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t x = __byte_perm(a, b, h ? 0x7362 : 0x5140);  // bytes a, b, a, b of neighbouring positions
-      if constexpr (Format<kFormat>::kBits == 8) {
-        uint32_t hi, lo;
-        split_bytes<kFormat>(x, hi, lo);
-        out[2 * h] = scaled<kRare>(__byte_perm(lo, hi, 0x5140), f, rest);
-        out[2 * h + 1] = scaled<kRare>(__byte_perm(lo, hi, 0x7362), f, rest);
-      } else {
-        uint32_t he, le, ho, lo;
-        split_nibbles(x, he, le, ho, lo);
-        out[4 * h] = scaled<kRare>(__byte_perm(le, he, 0x5140), f, rest);
-        out[4 * h + 1] = scaled<kRare>(__byte_perm(lo, ho, 0x5140), f, rest);
-        out[4 * h + 2] = scaled<kRare>(__byte_perm(le, he, 0x7362), f, rest);
-        out[4 * h + 3] = scaled<kRare>(__byte_perm(lo, ho, 0x7362), f, rest);
-      }
-    }
-  }
+  constexpr int kHalf = 16 / Format<kFormat>::kBits;  // elements of half a word
+  // halves of the two words side by side: the key's pairs of such a word are the wanted ones
+  key_word<kFormat, kRare>(__byte_perm(a, b, 0x5410), f, rest, out);
+  key_word<kFormat, kRare>(__byte_perm(a, b, 0x7632), f, rest, out + kHalf);
 }
 
 // ---- launches --------------------------------------------------------------------------------------------------------

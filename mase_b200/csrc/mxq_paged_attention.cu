@@ -130,7 +130,7 @@ struct Shape {
   static __host__ __device__ constexpr int value_turn(int i) {
     return kRow == 128 ? ((i >> 8) & 3) << 5 : (kRow == 256 ? ((i >> 9) & 3) << 5 : (kRow == 512 ? ((i >> 10) & 3) << 5 : 0));
   }
-  static constexpr int kStages = kRow <= 64 ? 4 : (kRow <= 128 ? 2 : 2);
+  static constexpr int kStages = kRow <= 64 ? 4 : 2;
 };
 // element (0 .. D-1) that half `half` of pair i of key word w of piece c of lane t holds
 template <int kFormat, int D>
@@ -161,6 +161,14 @@ __device__ __forceinline__ float exp2_fast(float x) {  // results below 2^-126 b
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+
+// Which tile a warp works on, for the few uses that need to know.
+struct Place {
+  int b, row, rows, tok;
+  __device__ __forceinline__ int64_t score_row(const AttnArgs &a) const {
+    return ((int64_t)b * rows + row) * a.score_tokens + tok;
+  }
+};
 
 template <typename T, int kFormat, int D, int NT>
 struct Worker {
@@ -222,14 +230,15 @@ struct Worker {
 
   // One tile from a stage of the ring; `live` tokens of it exist.
   template <bool kRare>
-  __device__ __forceinline__ void tile(const uint8_t *stage, int live, int bits, const AttnArgs &a, int64_t score_row,
-                                       int lane) {
+  __device__ __forceinline__ void tile(const uint8_t *stage, int live, int bits, const AttnArgs &a, const Place &at, int lane) {
     const float c_hi = a.c_hi, c_lo = a.c_lo;
     const int t = lane & 3, r = lane >> 2;
     const int offset = raw_offset<kFormat>(bits);
-    float s[NT][4];
+    float s[NT][4], s_odd[NT][4];  // two chains of products: even and odd steps
 #pragma unroll
-    for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] = s_odd[n][i] = 0.f;
 #pragma unroll
     for (int c = 0; c < S::kKeyPieces; ++c) {
       uint32_t pairs[2][S::kKeyWords * S::kPairs];
@@ -254,9 +263,14 @@ struct Worker {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int z = kTerms - 1; z >= 0; --z)
-            mma(s[n], rows, q[z][c * kStepsHere + k][n][0], q[z][c * kStepsHere + k][n][1]);
+            mma((c * kStepsHere + k) & 1 ? s_odd[n] : s[n], rows, q[z][c * kStepsHere + k][n][0],
+                q[z][c * kStepsHere + k][n][1]);
       }
     }
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[n][i] += s_odd[n][i];
     // rows: tokens r (entries 0, 1) and r + 8 (2, 3); columns: heads 2t, 2t + 1
     float x[NT][4], top = kLowest;
 #pragma unroll
@@ -275,7 +289,7 @@ struct Worker {
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, x[n][i]);
     if (a.scores != nullptr) {
-      float *scores = a.scores + score_row * (8 * NT);
+      float *scores = a.scores + at.score_row(a) * (8 * NT);
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -471,7 +485,7 @@ __device__ __forceinline__ bool any_rare(uint32_t w, int bits) {
 }
 
 template <typename T, int kFormat, int D, int NT>
-__global__ void __launch_bounds__(kWarps * 32, Elem<T>::kBf16 && D == 128 && NT == 1 ? 4 : 1)
+__global__ void __launch_bounds__(kWarps * 32, Elem<T>::kBf16 && D == 128 && NT == 1 ? 3 : 1)
 attention_kernel(const Cache c, const Table table, const AttnArgs a) {
   using S = Shape<kFormat, D>;
   constexpr int kHeads = 8 * NT;
@@ -501,16 +515,15 @@ attention_kernel(const Cache c, const Table table, const AttnArgs a) {
     here.unit = (int)(in_seq - (int64_t)here.row * here.units);
   }
 
-  // Where the warp's tiles lie is worked out for 32 units at a time, one per lane: `place` is the byte offset of the
-  // lane's tile (of the batch of units in use) from the start of the pages, `entry` and `entry_off` are the page table
+  // Where the warp's tiles lie is worked out for 32 units at a time, one per lane: `place` is the offset of the
+  // lane's tile (of the batch of units in use) from the start of the pages in units of 16 bytes, `entry` and `entry_off` are the page table
   // entry and the offset inside the page for the batch after it, whose loads have 32 units of time to arrive.
   Cursor ahead = here;  // first unit of the batch that is looked up next
   int looked_up = 0;    // units looked up
   int entry = 0;
   uint32_t entry_off = 0;
-  uint64_t place = 0;
+  uint32_t place = 0;
   constexpr uint32_t kNoTile = 0xFFFFFFFFu;
-  constexpr uint64_t kNoPlace = ~0ull;
   const uint32_t page_bytes = (uint32_t)(c.heads << c.page_log2) * S::kRow;  // below 2^32: at most 32767 heads
   auto look_up = [&]() {
     Cursor mine = ahead;
@@ -540,23 +553,36 @@ attention_kernel(const Cache c, const Table table, const AttnArgs a) {
     }
   };
   auto settle = [&]() {
-    place = kNoPlace;
+    place = kNoTile;
     if (entry_off != kNoTile) {
       if (entry < 0 || entry >= c.pages)
         report(a.status);
       else
-        place = (uint64_t)(uint32_t)entry * page_bytes + entry_off;
+        place = (uint32_t)(((uint64_t)(uint32_t)entry * page_bytes + entry_off) >> 4);  // the host bounds it
     }
   };
   const int key_to = S::key_slot(lane * 16 / S::kRow, lane * 16 % S::kRow);
   const int value_to = S::value_slot(lane * 16 / S::kRow, lane * 16 % S::kRow);
+  const uint8_t *k_base = c.codes[0] + lane * 16, *v_base = c.codes[1] + lane * 16;
+  // scale bytes: 4 to a lane, first those of the key rows, then those of the value rows (head_dim 256: one after the other)
+  constexpr int kScaleWords = 4 * S::kScaleRow;  // of one side
+  const bool value_scales = kScaleWords < 32 && lane >= kScaleWords;
+  const uint8_t *s_base = (value_scales ? c.scales[1] : c.scales[0]) + (lane - (value_scales ? kScaleWords : 0)) * 4;
+  const int64_t to_value_scales = c.scales[1] - c.scales[0];
+  auto copy_scales = [&](uint8_t *dst, const uint8_t *sp) {
+    if constexpr (kScaleWords == 32) {
+      copy_async<4>(dst + lane * 4, sp), copy_async<4>(dst + S::kScaleBytes + lane * 4, sp + to_value_scales);
+    } else {
+      if (lane < 2 * kScaleWords) copy_async<4>(dst + lane * 4, sp);
+    }
+  };
   uint32_t absent = 0;  // bit s: the tile in stage s does not exist
   auto issue = [&](int unit, int stage) {  // copies the warp's tile of a unit of the batch in use
-    const uint64_t off = __shfl_sync(0xFFFFFFFFu, place, unit & 31);
-    if (off != kNoPlace) {
+    const uint32_t off = __shfl_sync(0xFFFFFFFFu, place, unit & 31);
+    if (off != kNoTile) {
       absent &= ~(1u << stage);
       uint8_t *dst = ring + stage * S::kStage;
-      const uint8_t *kp = c.codes[0] + off + lane * 16, *vp = c.codes[1] + off + lane * 16;
+      const uint8_t *kp = k_base + (uint64_t)off * 16, *vp = v_base + (uint64_t)off * 16;
 #pragma unroll
       for (int i = 0; i < S::kSide; i += 512)
         if (S::kSide % 512 == 0 || lane * 16 < S::kSide) {
@@ -564,14 +590,9 @@ attention_kernel(const Cache c, const Table table, const AttnArgs a) {
           copy_async<16>(dst + S::kSide + i + (value_to ^ S::value_turn(i)), vp + i);
         }
       if constexpr (kFormat != MXQ_CACHE_BF16) {
-        constexpr int kPerScale = S::kRow / S::kScaleRow;  // code bytes of a block: 32 or 16
-#pragma unroll
-        for (int i = 0; i < 8 * S::kScaleRow; i += 32) {
-          const int word = i + lane, side = word >= 4 * S::kScaleRow;
-          if (8 * S::kScaleRow % 32 == 0 || word < 8 * S::kScaleRow)
-            copy_async<4>(dst + 2 * S::kSide + word * 4,
-                          (side ? c.scales[1] : c.scales[0]) + (word - side * 4 * S::kScaleRow) * 4 + off / kPerScale);
-        }
+        constexpr int kScalesPer16 = 16 * 8 / S::kBits;  // elements of 16 code bytes; one scale byte for 32
+        const uint8_t *sp = s_base + (kScalesPer16 == 32 ? (uint64_t)off : (uint64_t)(off >> 1));
+        copy_scales(dst + 2 * S::kSide, sp);
       }
     } else {
       absent |= 1u << stage;
@@ -623,7 +644,7 @@ attention_kernel(const Cache c, const Table table, const AttnArgs a) {
     const int live = here.length - tok;
     if ((absent >> stage) & 1u) {  // behind the end, or the page does not exist: its tokens are left out
       if (a.scores != nullptr) {
-        float *sc = a.scores + (((int64_t)here.b * rows + here.row) * a.score_tokens + tok) * kHeads;
+        float *sc = a.scores + Place{here.b, here.row, rows, tok}.score_row(a) * kHeads;
         for (int j = lane; j < min(live, kTile) * kHeads; j += 32) sc[j] = -INFINITY;
       }
     } else {
@@ -637,9 +658,9 @@ attention_kernel(const Cache c, const Table table, const AttnArgs a) {
         rare = __any_sync(0xFFFFFFFFu, rare);
       }
       if (kFormat != MXQ_CACHE_BF16 && rare)
-        w.template tile<true>(st, live, c.bits, a, ((int64_t)here.b * rows + here.row) * a.score_tokens + tok, lane);
+        w.template tile<true>(st, live, c.bits, a, Place{here.b, here.row, rows, tok}, lane);
       else
-        w.template tile<false>(st, live, c.bits, a, ((int64_t)here.b * rows + here.row) * a.score_tokens + tok, lane);
+        w.template tile<false>(st, live, c.bits, a, Place{here.b, here.row, rows, tok}, lane);
     }
     stage = stage == S::kStages - 1 ? 0 : stage + 1;
     if (i + 1 == todo) let_next_start();
@@ -712,14 +733,13 @@ attention_kernel(const Cache c, const Table table, const AttnArgs a) {
 
 // Joins the parts of the rows that CTAs share, and adds the softmax weights of every token to the caller's statistics:
 //   weights[b, head, j] += sum over the group of exp(s_j - m) / l.
-// grid: (x, heads, batch): heads g of a group with g % x == blockIdx.x are joined by the CTA, tokens are strided over x.
+// grid: (x, heads, batch): the x CTAs' warps take the heads of the group in turn, and their threads the tokens.
 // Before the wait only what the attention kernel does not write is read: its CTAs let this kernel start after their own
 // wait, so everything before it in the stream has finished.
 template <typename T>
 __global__ void __launch_bounds__(kFinishThreads)
 finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
-  extern __shared__ float4 sm[];  // [kFinishThreads], then [group] pairs of maximum and 1 / sum
-  float2 *stats = reinterpret_cast<float2 *>(sm + kFinishThreads);
+  extern __shared__ float2 stats[];  // [group] pairs of maximum and 1 / sum
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int head = blockIdx.y, b = blockIdx.z;
   const int rows = heads * a.head_tiles;
@@ -756,36 +776,40 @@ finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
   };
   int first, last;
   bool late;
-  locate(blockIdx.x, first, last, late);
+  const int warps = gridDim.x * (kFinishThreads / 32), g_first = blockIdx.x * (kFinishThreads / 32) + warp;
+  locate(min(g_first, a.group - 1), first, last, late);
   wait_for_previous();
 
-  const int vecs = dim >> 2, groups = kFinishThreads / vecs, vec = tid & (vecs - 1), group = tid / vecs;
-  for (int g = blockIdx.x; g < a.group; g += gridDim.x) {
-    if (g != blockIdx.x) locate(g, first, last, late);
+  // One warp for a head.  A part is dim / 4 vectors: lanes beyond that take further parts, to be added up at the end.
+  const int vecs = dim >> 2;
+  for (int g = g_first; g < a.group; g += warps) {
+    if (g != g_first) locate(g, first, last, late);
     if (first == last) continue;  // finished by its CTA
     const float2 st = join(g, first, last, late);
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = first + group; c <= last; c += groups) {
-      const int64_t part = part_of(c, first, late, g);
-      const float f = exp2f(a.part_ml[part].x - st.x);
-      const float4 o = reinterpret_cast<const float4 *>(a.part_o + part * dim)[vec];
-      v.x += f * o.x, v.y += f * o.y, v.z += f * o.z, v.w += f * o.w;
-    }
-    sm[tid] = v;
-    __syncthreads();
-    if (tid < vecs) {
-      for (int k = 1; k < groups; ++k) {
-        const float4 o = sm[k * vecs + tid];
-        v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+    for (int v0 = 0; v0 < vecs; v0 += 32) {  // more than once for head_dim 256
+      const int at_once = vecs < 32 ? 32 / vecs : 1, vec = v0 + (vecs < 32 ? lane & (vecs - 1) : lane);
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+      for (int c = first + (vecs < 32 ? lane / vecs : 0); c <= last; c += at_once) {
+        const int64_t part = part_of(c, first, late, g);
+        const float f = exp2f(a.part_ml[part].x - st.x);
+        const float4 o = reinterpret_cast<const float4 *>(a.part_o + part * dim)[vec];
+        v.x += f * o.x, v.y += f * o.y, v.z += f * o.z, v.w += f * o.w;
       }
-      const float f = st.y == 0.f ? 0.f : 1.f;
-      T *out = static_cast<T *>(a.out) + ((int64_t)b * a.q_heads + head * a.group + g) * dim + 4 * tid;
-      const float r[4] = {f == 0.f ? 0.f : v.x / st.y, f == 0.f ? 0.f : v.y / st.y, f == 0.f ? 0.f : v.z / st.y,
-                          f == 0.f ? 0.f : v.w / st.y};
-      store_vals(out, 0, r);
+      for (int x = 16; x >= vecs; x >>= 1) {
+        v.x += __shfl_xor_sync(0xFFFFFFFFu, v.x, x), v.y += __shfl_xor_sync(0xFFFFFFFFu, v.y, x);
+        v.z += __shfl_xor_sync(0xFFFFFFFFu, v.z, x), v.w += __shfl_xor_sync(0xFFFFFFFFu, v.w, x);
+      }
+      const float r[4] = {v.x / st.y, v.y / st.y, v.z / st.y, v.w / st.y};
+      const float none[4] = {0.f, 0.f, 0.f, 0.f};
+      T *out = static_cast<T *>(a.out) + ((int64_t)b * a.q_heads + head * a.group + g) * dim + 4 * vec;
+      if (vecs >= 32 || lane < vecs) {
+        if (st.y == 0.f)
+          store_vals(out, 0, none);
+        else
+          store_vals(out, 0, r);
+      }
     }
-    __syncthreads();
   }
   if (a.weights == nullptr) return;
   for (int g = warp; g < a.group; g += kFinishThreads / 32) {
@@ -934,6 +958,8 @@ int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, 
   if (weights && weights_width < 1) return MXQ_ERR_SHAPE;
   const int dim = cache->head_dim;
   const int64_t tokens = table_width << c.page_log2;
+  if (cache->pages * ((int64_t)c.heads << c.page_log2) * row_bytes_of(cache->format, dim) > MXQ_CACHE_SIDE_BYTES)
+    return MXQ_ERR_SHAPE;  // tiles are addressed by 32-bit multiples of 16 bytes
   const int nt = tiles_per_row(dtype, dim, group);
   int64_t most_ctas;
   const Workspace w = workspace_of(nt, batch, c.heads, q_heads, dim, tokens, weights != nullptr, most_ctas);
@@ -965,14 +991,15 @@ int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, 
   rc = dtype == MXQ_BF16 ? launch_attention<__nv_bfloat16>(cache->format, dim, c, t, a, nt, most_ctas, st)
                          : launch_attention<float>(cache->format, dim, c, t, a, nt, most_ctas, st);
   if (rc != MXQ_OK || (!parts && !weights)) return rc;
-  int64_t x = group;
+  int64_t x = (group + kFinishThreads / 32 - 1) / (kFinishThreads / 32);
   if (weights) {  // enough CTAs for the tokens, and no more than the GPU holds at once
     const int64_t need = (tokens + kFinishThreads - 1) / kFinishThreads;
     const int64_t cap = ((int64_t)gemm::sm_count() * 16 + c.heads * batch - 1) / (c.heads * batch);
-    x = need < cap ? need : cap;
+    const int64_t most = need < cap ? need : cap;
+    x = most > x ? most : x;
   }
   const dim3 grid((unsigned)x, (unsigned)c.heads, (unsigned)batch);
-  const size_t smem = kFinishThreads * 16 + (weights ? group * sizeof(float2) : 0);
+  const size_t smem = weights ? group * sizeof(float2) : 0;
   return dtype == MXQ_BF16
              ? launch_chained(finish_kernel<__nv_bfloat16>, grid, kFinishThreads, smem, st, 1, a, c.heads, 8 * nt, dim)
              : launch_chained(finish_kernel<float>, grid, kFinishThreads, smem, st, 1, a, c.heads, 8 * nt, dim);
