@@ -5,7 +5,7 @@ Public surface (same names as in `chop.nn.quantizers` / `chop.nn.quantized`):
   modules:    LinearMXFP, LinearMXInt, LinearBlockFP, linearBlockFP, EmbeddingMXFP / MXInt, RMSNormMinifloat,
               AttentionMXFP / MXInt (+ the Qwen3 variants), GatedMLPMX            (mase_b200.attention)
   functional: matmul / bmm / kv_cache / softmax / silu / rope for mxfp, mxint, minifloat
-  kv cache:   PagedKVCache (MX or bf16 pages), paged_kv_append / _gather / _evict, paged_attention  (mase_b200.kv_cache)
+  kv cache:   PagedKVCache, PagedKVState (MX or bf16 pages), paged_kv_append / _gather / _evict, paged_attention  (mase_b200.kv_cache)
   calibration: the clipping search inside *_quantizer_sim(quantile_search=True); GPTQ (mase_b200.gptq)
   patch(chop) registers them in an imported MASE so that its quantize passes pick them up.
 
@@ -48,7 +48,7 @@ from .attention import (  # noqa: F401
     AttentionMXFP, AttentionMXInt, GatedMLPMX, Qwen3AttentionMXFP, Qwen3AttentionMXInt,
 )
 from .kv_cache import (  # noqa: F401
-    PagedKVCache, paged_attention, paged_kv_append, paged_kv_evict, paged_kv_gather,
+    PagedKVCache, PagedKVState, paged_attention, paged_kv_append, paged_kv_evict, paged_kv_gather,
 )
 from .patch import patch  # noqa: F401
 

@@ -12,6 +12,10 @@ queries, probabilities and cached keys / values, the quantizer + fp32 softmax (`
 products as one batched launch each (`mxq_gemm_dense_batched`: Q K^T over batch x heads with K = head_dim, P V with
 K = the key length).  One operand of each product is unquantized in the reference (keys, values), so fp32 tensors go
 through the split that keeps fp32-level products; bf16 products are exact.
+
+`past_key_value` is anything with the `update` of a key/value cache, or a `mase_b200.kv_cache.PagedKVState`: then keys and
+values are quantized into pages, and a step of one new token per sequence runs on the pages themselves when softmax and
+probabilities are not quantized and no mask is given (its second return value is then None).
 """
 
 from __future__ import annotations
@@ -21,6 +25,7 @@ from torch import Tensor, nn
 
 from . import functional as F_mx
 from .gemm import batched_product
+from .kv_cache import PagedKVState
 from .modules import forward_siblings
 from .quantizers import mxfp_quantizer, mxint_quantizer
 
@@ -141,8 +146,18 @@ class _AttentionMX(nn.Module):
             query, key = F_mx.rope_minifloat(query, key, cos, sin, self.rope_config)
         else:
             query, key = F_mx._apply_rope(query, key, cos, sin, 1)
+        paged = past_key_value if isinstance(past_key_value, PagedKVState) else None
+        if paged is not None:  # quantizes what it stores
+            paged.check_format(self.layer_idx, None if self.kv_cache_bypass else self._format, self.kv_cache_config)
+            if (query.shape[2] == 1 and attention_mask is None and self.softmax_bypass and self.av_bypass
+                    and not (self.training and self.attention_dropout > 0)
+                    and not (torch.is_grad_enabled() and query.requires_grad)):
+                paged.append(key, value, self.layer_idx)
+                query = query if self.qk_bypass else self._quantize(query, self.qk_config)
+                out = paged.attend(query, self.layer_idx, self.scaling)  # [B, H, 1, D]
+                return self.o_proj(out.reshape(*input_shape, -1)), None
         if past_key_value is not None:
-            if not self.kv_cache_bypass:
+            if not self.kv_cache_bypass and paged is None:
                 key, value = self._kv_cache(key, value)
             key, value = past_key_value.update(key, value, self.layer_idx,
                                                {"sin": sin, "cos": cos, "cache_position": cache_position})
@@ -175,6 +190,8 @@ class _AttentionMX(nn.Module):
                 weights = nn.functional.dropout(weights, p=self.attention_dropout, training=True)
             if not self.av_bypass:
                 weights = self._quantize(weights, self.av_config)
+        if paged is not None:
+            paged.accumulate(weights, self.layer_idx)
         out = self._product(weights, value.transpose(2, 3).contiguous(), exact=False)  # [B, H, S, D]
         out = out.transpose(1, 2).contiguous().reshape(*input_shape, -1)
         return self.o_proj(out), weights

@@ -390,3 +390,104 @@ def paged_kv_evict(cache: PagedKVCache, page_table: Tensor, lengths: Tensor, wei
     _lib.check(rc, "mxq_paged_evict")
     _check_every_call(cache)
     return new_lengths, new_weights, new_positions
+
+
+class PagedKVState:
+    """The paged caches of a model's attention layers, with the page table, the lengths and (`track=True`) the statistics
+    that eviction needs.  The attention blocks of `mase_b200.attention` take it as `past_key_value`:
+
+        state = PagedKVState([PagedKVCache(...) for _ in layers], page_table)
+        block(hidden, (cos, sin), mask, past_key_value=state)   # every layer, layer_idx names its cache
+        state.advance(tokens)                                   # once per forward, when all layers have run
+
+    A block writes its new keys and values into the pages.  A single new token per sequence then attends over the pages
+    (`paged_attention`) when the block asks for nothing that needs the dense probabilities: no attention_mask, and softmax
+    and probabilities not quantized (`bypass` of "softmax" and "av_matmul").  Everything else, prompts above all, reads the
+    cached rows back as dense tensors.
+
+    counts (int32 [batch] or None): how many of the forward's tokens each sequence has (a right-padded batch); set it before
+    the forward, `advance` uses it and clears it.  max_length is the host's bound on the lengths: dense tensors are that
+    long (plus the new tokens)."""
+
+    def __init__(self, caches: list[PagedKVCache], page_table: Tensor, lengths: Tensor | None = None, max_length: int = 0,
+                 track: bool = False):
+        if not caches:
+            raise ValueError("PagedKVState needs the cache of at least one layer")
+        first = caches[0]
+        for c in caches:
+            if (c.num_kv_heads, c.page_size, c.device) != (first.num_kv_heads, first.page_size, first.device):
+                raise ValueError("the layers' caches have the same heads and page size and are on one device")
+        self.caches, self.page_table = list(caches), page_table
+        if lengths is None:
+            lengths = torch.zeros(page_table.shape[0], dtype=torch.int32, device=first.device)
+        batch = _check_table(first, page_table, lengths)
+        self.lengths, self.max_length, self.counts = lengths, max_length, None
+        self.capacity = page_table.shape[1] * first.page_size
+        self.next_position = lengths.clone()  # positions count evicted tokens too
+        self.weights = self.positions = None
+        if track:
+            shape = (batch, first.num_kv_heads, self.capacity)
+            slots = torch.arange(self.capacity, dtype=torch.int32, device=first.device).expand(shape)
+            self.weights = [torch.zeros(shape, dtype=torch.float32, device=first.device) for _ in caches]
+            self.positions = [slots.contiguous() for _ in caches]
+        self._after = None  # (tokens, lengths after the forward that is under way)
+
+    def check_format(self, layer_idx: int, fmt: str | None, config: dict | None) -> None:
+        """Raises unless the layer's cache has the format that a block's `kv_cache` entry asks for."""
+        c = self.caches[layer_idx]
+        if (c._code, c._bits) != _format_of(fmt, config):
+            raise ValueError(f"layer {layer_idx}: the block's kv_cache configuration is not the format of its paged cache")
+
+    def lengths_after(self, tokens: int) -> Tensor:
+        if self._after is None or self._after[0] != tokens:
+            if self.max_length + tokens > self.capacity:
+                raise ValueError(f"{self.max_length} + {tokens} tokens do not fit a page table of {self.capacity}")
+            self._after = (tokens, self.lengths + (tokens if self.counts is None else self.counts))
+        return self._after[1]
+
+    def append(self, key: Tensor, value: Tensor, layer_idx: int) -> None:
+        self.lengths_after(key.shape[2])  # checks the room
+        tracked = {} if self.positions is None else {"positions": self.positions[layer_idx],
+                                                     "next_position": self.next_position}
+        paged_kv_append(self.caches[layer_idx], key, value, self.page_table, self.lengths, self.counts, **tracked)
+
+    def update(self, key: Tensor, value: Tensor, layer_idx: int, cache_kwargs=None) -> tuple[Tensor, Tensor]:
+        """Write new keys and values and return all cached ones as dense tensors (the call of a key/value cache)."""
+        self.append(key, value, layer_idx)
+        tokens = key.shape[2]
+        return paged_kv_gather(self.caches[layer_idx], self.page_table, self.lengths_after(tokens), self.max_length + tokens,
+                               key.dtype)
+
+    def attend(self, query: Tensor, layer_idx: int, scaling: float | None = None) -> Tensor:
+        """`paged_attention` of the token that has just been appended; accumulates its weights when tracking."""
+        return paged_attention(self.caches[layer_idx], query, self.page_table, self.lengths_after(1), scaling,
+                               None if self.weights is None else self.weights[layer_idx])
+
+    def accumulate(self, probabilities: Tensor, layer_idx: int) -> None:
+        """Add dense softmax weights [batch, heads, tokens, keys] of the forward's tokens to the statistics."""
+        if self.weights is None:
+            return
+        b, h, t, n = probabilities.shape
+        heads = self.caches[layer_idx].num_kv_heads
+        p = probabilities.detach().float()
+        if self.counts is not None:  # rows of padding count for nothing
+            live = torch.arange(t, device=p.device) < self.counts[:, None]
+            p = torch.where(live[:, None, :, None], p, 0.0)
+        self.weights[layer_idx][:, :, :n] += p.view(b, heads, h // heads, t, n).sum((2, 3))
+
+    def advance(self, tokens: int) -> None:
+        """The forward's tokens are now cached in every layer."""
+        after = self.lengths_after(tokens)
+        new = tokens if self.counts is None else self.counts
+        self.lengths, self.next_position = after, self.next_position + new
+        self.max_length += tokens
+        self.counts = self._after = None
+
+    def evict(self, keep: int, recent: int = 0) -> None:
+        """`paged_kv_evict` in every layer; needs `track=True`."""
+        if self.weights is None:
+            raise RuntimeError("eviction needs the statistics of a PagedKVState with track=True")
+        for i, cache in enumerate(self.caches):
+            lengths, self.weights[i], self.positions[i] = paged_kv_evict(
+                cache, self.page_table, self.lengths, self.weights[i], keep, recent, self.positions[i], self.next_position)
+        self.lengths, self.max_length, self._after = lengths, min(self.max_length, keep), None

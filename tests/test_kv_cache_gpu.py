@@ -499,6 +499,134 @@ def test_captured_steps_follow_their_tensors_and_share_nothing():
     gemm.check_status()
 
 
+class ListCache:
+    """The part of a dense key/value cache the attention block uses."""
+
+    def __init__(self):
+        self.k, self.v = {}, {}
+
+    def update(self, k, v, layer_idx, cache_kwargs=None):
+        self.k[layer_idx] = k if layer_idx not in self.k else torch.cat([self.k[layer_idx], k], dim=-2)
+        self.v[layer_idx] = v if layer_idx not in self.v else torch.cat([self.v[layer_idx], v], dim=-2)
+        return self.k[layer_idx], self.v[layer_idx]
+
+
+def blocks(name, dtype, bypass, layers=2, seed=5):
+    """Attention blocks of hidden 128, 8 heads of 32 over 2 key/value heads; `bypass`: softmax and probabilities plain."""
+    fmt, cfg = CONFIGS[name]
+    mini = {"data_in_exponent_width": 5, "data_in_frac_width": 10}
+    q = {"rope": mini, "qk_matmul": cfg or {"bypass": True}, "kv_cache": cfg or {"bypass": True},
+         "softmax": {"bypass": True} if bypass else mini, "av_matmul": {"bypass": True} if bypass else cfg}
+    cls = mb.AttentionMXInt if fmt == "mxint" else mb.AttentionMXFP
+    torch.manual_seed(seed)
+    made = [cls(None, i, q, hidden_size=128, num_heads=8, num_kv_heads=2, head_dim=32, dtype=dtype) for i in range(layers)]
+    return [m.to(DEV).eval() for m in made]
+
+
+def rope(start, n, batch, dtype):
+    pos = torch.as_tensor(start).view(-1, 1) + torch.arange(n)
+    ang = pos[..., None] * (1.0 / 10000 ** (torch.arange(0, 32, 2) / 32))
+    ang = torch.cat([ang, ang], -1).expand(batch, n, 32)
+    return ang.cos().to(dtype).to(DEV), ang.sin().to(dtype).to(DEV)
+
+
+def causal(n, past, batch, dtype):
+    m = torch.full((n, past + n), torch.finfo(dtype).min).triu(past + 1).to(dtype)
+    return m.expand(batch, 1, n, past + n).contiguous().to(DEV)
+
+
+@pytest.mark.parametrize("name,dtype,bypass", [("e4m3", torch.float32, True), ("e4m3", torch.bfloat16, True),
+                                               ("int8", torch.float32, True), ("none", torch.bfloat16, True),
+                                               ("e4m3", torch.float32, False), ("e2m1", torch.float32, True)])
+def test_attention_blocks_on_a_paged_cache(name, dtype, bypass):
+    """A prompt, its continuation as a second chunk, and single tokens through two blocks: the same outputs as with a dense
+    cache of fake-quantized keys and values.  fp32: both sides round only in fp32, over at most 96 keys; the tensor-core
+    products and the softmax are each good to about 2**-18 of the largest value.  bf16: the dense side rounds scores and
+    probabilities to bf16 (2**-8 of a score of magnitude up to 8 moves a probability by 3 %, weights that sum to one)."""
+    batch, heads, page, width = 2, 2, 16, 6
+    fmt, cfg = CONFIGS[name]
+    layers = blocks(name, dtype, bypass)
+    caches = [mb.PagedKVCache(batch * width + 1, heads, 32, page, fmt, cfg, DEV) for _ in layers]
+    table = torch.randperm(batch * width, generator=torch.Generator().manual_seed(1)).view(batch, width).int().to(DEV)
+    state, dense = mb.PagedKVState(caches, table, track=True), ListCache()
+    # quantized probabilities come in blocks of 32 keys, in the dense block as well
+    sizes, past = [33, 32, 1, 1, 1] if bypass else [32, 64], 0
+    with torch.no_grad():
+        for i, n in enumerate(sizes):
+            h1 = h2 = rows(batch, n, 128, seed=40 + i, dtype=dtype, spread=0.1).to(DEV)
+            cs = rope(past, n, batch, dtype)
+            mask = causal(n, past, batch, dtype)
+            for layer in layers:
+                # the last step of the paged side runs with a mask, that is on dense tensors
+                o1, p1 = layer(h1, cs, mask if n > 1 or i == 4 else None, past_key_value=state)
+                o2, p2 = layer(h2, cs, mask, past_key_value=dense)
+                assert (p1 is None) == (n == 1 and i < 4 and bypass)
+                tol = 2e-4 if dtype == torch.float32 else 4e-2
+                if not bypass:
+                    tol = 2e-2  # a probability that lands on the other side of a rounding border
+                err = float((o1.float() - o2.float()).abs().max() / o2.float().abs().max())
+                assert err <= tol, (name, i, err)
+                h1, h2 = o1, o2
+                if dtype == torch.bfloat16 or not bypass:
+                    h1 = h2  # compare layer by layer, not what errors grow into
+            state.advance(n)
+            past += n
+    gemm.check_status()
+    assert state.lengths.tolist() == [past, past] == state.next_position.tolist()
+    for w in state.weights:  # one unit of weight for every query of every head of a group
+        assert torch.allclose(w.sum(-1), torch.full((batch, heads), 4.0 * past, device=DEV), rtol=3e-2 if dtype == torch.bfloat16 or not bypass else 1e-5)
+    state.evict(40, 8)
+    assert state.lengths.tolist() == [40, 40] and state.max_length == 40
+    for w, pos in zip(state.weights, state.positions):
+        assert bool((w[..., 40:] == 0).all()) and bool((pos[..., 40:] == -1).all())
+        for x in pos[..., :40].reshape(-1, 40).tolist():
+            assert len(set(x)) == 40 and set(range(past - 8, past)) <= set(x)
+    if not bypass:
+        return
+    with torch.no_grad():
+        h = rows(batch, 1, 128, seed=60, dtype=dtype).to(DEV)
+        for layer in layers:
+            out, _ = layer(h, rope(past, 1, batch, dtype), None, past_key_value=state)
+        state.advance(1)
+    assert bool(torch.isfinite(out).all()) and state.lengths.tolist() == [41, 41]
+    assert state.positions[0][:, :, 40].unique().tolist() == [past]
+    gemm.check_status()
+
+
+def test_padded_prompts_and_refusals_of_the_state():
+    layers = blocks("int8", torch.float32, True, layers=1)
+    fmt, cfg = CONFIGS["int8"]
+    cache = mb.PagedKVCache(9, 2, 32, 16, fmt, cfg, DEV)
+    table = torch.arange(8, dtype=torch.int32, device=DEV).view(2, 4)
+    state = mb.PagedKVState([cache], table, track=True)
+    h = rows(2, 20, 128, seed=3, dtype=torch.float32, spread=0.1).to(DEV)
+    with torch.no_grad():
+        state.counts = i32([20, 13])
+        layers[0](h, rope(0, 20, 2, torch.float32), causal(20, 0, 2, torch.float32), past_key_value=state)
+        state.advance(20)
+        assert state.lengths.tolist() == [20, 13] and state.max_length == 20 and state.counts is None
+        assert torch.allclose(state.weights[0].sum(-1).cpu(), torch.tensor([[80.0, 80.0], [52.0, 52.0]]), rtol=1e-5)
+        step = rows(2, 1, 128, seed=4, dtype=torch.float32, spread=0.1).to(DEV)
+        out, _ = layers[0](step, rope([20, 13], 1, 2, torch.float32), None, past_key_value=state)
+        # the shorter sequence by itself
+        alone = mb.PagedKVState([mb.PagedKVCache(9, 2, 32, 16, fmt, cfg, DEV)], table[1:])
+        layers[0](h[1:, :13], rope(0, 13, 1, torch.float32), causal(13, 0, 1, torch.float32), past_key_value=alone)
+        alone.advance(13)
+        one, _ = layers[0](step[1:], rope(13, 1, 1, torch.float32), None, past_key_value=alone)
+    assert float((out[1:] - one).abs().max() / one.abs().max()) <= 1e-5
+    with pytest.raises(RuntimeError, match="track"):
+        alone.evict(4)
+    with pytest.raises(ValueError, match="fit"):
+        state.lengths_after(60)
+    with pytest.raises(ValueError, match="format"):
+        blocks("e4m3", torch.float32, True, layers=1)[0](step, rope(20, 1, 2, torch.float32), None, past_key_value=state)
+    with pytest.raises(ValueError):
+        mb.PagedKVState([], table)
+    with pytest.raises(ValueError):
+        mb.PagedKVState([cache, mb.PagedKVCache(9, 2, 32, 32, fmt, cfg, DEV)], table)
+    gemm.check_status()
+
+
 def test_calls_without_the_compiled_binding(monkeypatch):
     """The same C calls through ctypes, arguments that need a copy among them."""
     from mase_b200 import kv_cache
