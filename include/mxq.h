@@ -392,7 +392,9 @@ int mxq_mx_linear_static(const void *x, int in_dtype, const uint8_t *w_codes, co
  *   MXQ_CACHE_E5M2     the same with 5 exponent and 2 fraction bits
  *   MXQ_CACHE_E2M1X2   D/2 bytes, MXFP4 codes, element 2i in the low nibble of byte i
  *   MXQ_CACHE_INT8     D int8 MXINT mantissas of `bits` bits (mxq_mxint_extract), biased shared exponents
- * Token i of sequence b lives in slot i % page_size of page page_table[b * table_stride + i / page_size].
+ * Token i of sequence b lives in slot i % page_size of page page_table[b * table_stride + i / page_size]; a table holds
+ * at most 2^30 tokens.  A page that several sequences name is read by all of them; rows are appended to and evicted from
+ * pages of one sequence only.
  *
  * Page tables and lengths are device memory and are only looked at on the device, so a captured launch follows their
  * contents.  An entry that is needed and lies outside [0, pages), a length that is negative or does not fit the table

@@ -6,6 +6,7 @@
 namespace mxq {
 namespace paged {
 
+constexpr int kMostTokens = 1 << 30;  // of a page table: token counts and what lies a few units behind fit 32 bits
 constexpr int kStatusBadPage = 8;  // a page table entry or a length points outside of the cache
 
 // Geometry of one cache; sides: 0 = keys, 1 = values.
@@ -51,7 +52,7 @@ inline int read_cache(const mxq_paged_cache *c, Cache &out) {
 inline int read_table(const int32_t *table, int64_t width, int64_t stride, int64_t batch, int page_log2) {
   if (!table) return MXQ_ERR_NULL;
   if (width < 1 || stride < 0 || (batch > 1 && stride < width)) return MXQ_ERR_SHAPE;
-  if (batch < 0 || batch > 65535 || width > (INT32_MAX >> page_log2)) return MXQ_ERR_SHAPE;
+  if (batch < 0 || batch > 65535 || width > (kMostTokens >> page_log2)) return MXQ_ERR_SHAPE;
   return MXQ_OK;
 }
 

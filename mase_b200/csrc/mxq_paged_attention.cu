@@ -51,8 +51,9 @@ struct AttnArgs {
   float *part_o;   // [ctas, 2, 8 * NT, dim]: unnormalised results of the rows a CTA shares with others
   float2 *part_ml; // [ctas, 2, 8 * NT]: their maximum and sum
   float2 *stats;   // [batch, q_heads] maximum and sum of rows of one CTA, when weights are accumulated
-  float *scores;   // [batch, heads, head_tiles, tokens, 8 * NT] when weights are accumulated
+  float *scores;   // [batch, heads, head_tiles, tokens, score_heads] when weights are accumulated
   int64_t score_tokens;
+  int score_heads; // heads of a tile that are kept: 2, 4, 8 or 16
   float *weights;
   int64_t weights_width;
   int *status;
@@ -289,13 +290,13 @@ struct Worker {
 #pragma unroll
       for (int i = 0; i < 4; ++i) top = fmaxf(top, x[n][i]);
     if (a.scores != nullptr) {
-      float *scores = a.scores + at.score_row(a) * (8 * NT);
+      float *scores = a.scores + at.score_row(a) * a.score_heads;
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int h = 0; h < 2; ++h)
-          if (r + 8 * h < live)
-            *reinterpret_cast<float2 *>(scores + (int64_t)(r + 8 * h) * (8 * NT) + n * 8 + 2 * t) =
+          if (r + 8 * h < live && n * 8 + 2 * t < a.score_heads)
+            *reinterpret_cast<float2 *>(scores + (r + 8 * h) * a.score_heads + n * 8 + 2 * t) =
                 make_float2(score(s[n][2 * h], c_hi, c_lo, 0.f), score(s[n][2 * h + 1], c_hi, c_lo, 0.f));
     }
     if (__any_sync(0xFFFFFFFFu, top > kSlack)) {
@@ -398,9 +399,10 @@ struct Worker {
 // ---- split ---------------------------------------------------------------------------------------------------------------
 // The rows of a launch are (sequence, key/value head, head tile), each a run of units of kUnit tokens (at least one) and
 // kRowCost empty units, which stand for what beginning and ending a row costs.  The units of all rows in order are divided
-// evenly between the CTAs, whatever the lengths are: with total = q * ctas + r, CTA i takes q or (i < r) q + 1 of them.  A row inside one CTA is finished there; of a row that
-// several CTAs share each leaves an unnormalised part with its maximum and sum, and the finish kernel joins them in the
-// order of the CTAs.  A CTA shares at most its first and its last row, so there are two part slots per CTA.
+// evenly between the CTAs, whatever the lengths are: with total = q * ctas + r, CTA i takes q or (i < r) q + 1 of them.
+// A row inside one CTA is finished there; of a row that several CTAs share each leaves an unnormalised part with its
+// maximum and sum, and the finish kernel joins them in the order of the CTAs.  A CTA shares at most its first and its
+// last row, so there are two part slots per CTA.
 struct Split {
   int64_t q, r;
   __device__ __forceinline__ Split(int64_t total, int64_t ctas) {
@@ -644,8 +646,8 @@ attention_kernel(const Cache c, const Table table, const AttnArgs a) {
     const int live = here.length - tok;
     if ((absent >> stage) & 1u) {  // behind the end, or the page does not exist: its tokens are left out
       if (a.scores != nullptr) {
-        float *sc = a.scores + Place{here.b, here.row, rows, tok}.score_row(a) * kHeads;
-        for (int j = lane; j < min(live, kTile) * kHeads; j += 32) sc[j] = -INFINITY;
+        float *sc = a.scores + Place{here.b, here.row, rows, tok}.score_row(a) * a.score_heads;
+        for (int j = lane; j < min(live, kTile) * a.score_heads; j += 32) sc[j] = -INFINITY;
       }
     } else {
       const uint8_t *st = ring + stage * S::kStage;
@@ -818,17 +820,15 @@ finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
     if (lane == 0) stats[g] = make_float2(st.x, st.y == 0.f ? 0.f : 1.f / st.y);
   }
   __syncthreads();
-  const float *scores = a.scores + ((int64_t)b * rows + head * a.head_tiles) * a.score_tokens * tile_heads;
+  const float *scores = a.scores + ((int64_t)b * rows + head * a.head_tiles) * a.score_tokens * a.score_heads;
   float *weights = a.weights + ((int64_t)b * heads + head) * a.weights_width;
   for (int j = blockIdx.x * kFinishThreads + tid; j < length; j += gridDim.x * kFinishThreads) {
     float sum = 0.f;
-    for (int g0 = 0; g0 < a.group; g0 += 4) {  // four heads of a tile lie together
-      const int ht = g0 / tile_heads;
-      const float4 s = *reinterpret_cast<const float4 *>(scores + ((int64_t)ht * a.score_tokens + j) * tile_heads + (g0 - ht * tile_heads));
-      sum += exp2f(s.x - stats[g0].x) * stats[g0].y;
-      if (g0 + 1 < a.group) sum += exp2f(s.y - stats[g0 + 1].x) * stats[g0 + 1].y;
-      if (g0 + 2 < a.group) sum += exp2f(s.z - stats[g0 + 2].x) * stats[g0 + 2].y;
-      if (g0 + 3 < a.group) sum += exp2f(s.w - stats[g0 + 3].x) * stats[g0 + 3].y;
+    for (int g = 0; g < a.group; g += 2) {  // two heads of a tile lie together
+      const int ht = g / tile_heads;
+      const float2 s = *reinterpret_cast<const float2 *>(scores + ((int64_t)ht * a.score_tokens + j) * a.score_heads + (g - ht * tile_heads));
+      sum += exp2f(s.x - stats[g].x) * stats[g].y;
+      if (g + 1 < a.group) sum += exp2f(s.y - stats[g + 1].x) * stats[g + 1].y;
     }
     weights[j] += sum;
   }
@@ -841,6 +841,12 @@ constexpr int kMostPerSm = 8;  // CTAs of the attention kernel on one SM, at mos
 
 static int64_t units_of_launch(int64_t batch, int64_t rows, int64_t tokens) {
   return batch * rows * ((tokens + kUnit - 1) / kUnit + kRowCost);
+}
+// Heads of a tile whose scores are kept for the weights: all of them, or the group's rounded up to a power of two.
+static int score_heads(int nt, int64_t group) {
+  int n = 2;
+  while (n < group && n < 8 * nt) n *= 2;
+  return n;
 }
 struct Workspace {
   int64_t ml, o, stats, scores, total;  // byte offsets
@@ -858,7 +864,7 @@ static Workspace workspace_of(int nt, int64_t batch, int64_t heads, int64_t q_he
   w.o = parts ? up(most_ctas * 2 * 8 * nt * (int64_t)sizeof(float2)) : 0;
   w.stats = w.o + (parts ? up(most_ctas * 2 * 8 * nt * dim * 4) : 0);
   w.scores = w.stats + (weights ? up(batch * q_heads * (int64_t)sizeof(float2)) : 0);
-  w.total = w.scores + (weights ? batch * heads * head_tiles * tokens * (8 * nt) * 4 : 0);
+  w.total = w.scores + (weights ? batch * heads * head_tiles * tokens * score_heads(nt, q_heads / heads) * 4 : 0);
   return w;
 }
 
@@ -915,7 +921,7 @@ using namespace mxq::paged;
 static int check_attention(const mxq_paged_cache *cache, int64_t batch, int64_t q_heads, int64_t table_width, int page_log2,
                            int64_t &group) {
   if (batch < 0 || batch > 65535 || q_heads < 1 || q_heads > 65535 || q_heads % cache->heads) return MXQ_ERR_SHAPE;
-  if (table_width < 1 || table_width > (INT32_MAX >> page_log2)) return MXQ_ERR_SHAPE;
+  if (table_width < 1 || table_width > (kMostTokens >> page_log2)) return MXQ_ERR_SHAPE;
   group = q_heads / cache->heads;
   return group <= 4096 ? MXQ_OK : MXQ_ERR_SHAPE;  // the statistics of a group fit shared memory
 }
@@ -984,7 +990,7 @@ int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, 
   a.part_o = parts ? reinterpret_cast<float *>(ws + w.o) : nullptr;
   a.stats = weights ? reinterpret_cast<float2 *>(ws + w.stats) : nullptr;
   a.scores = weights ? reinterpret_cast<float *>(ws + w.scores) : nullptr;
-  a.score_tokens = tokens;
+  a.score_tokens = tokens, a.score_heads = score_heads(nt, group);
   a.weights = weights, a.weights_width = weights_width, a.status = status;
   const Table t{page_table, table_stride, table_width};
   cudaStream_t st = (cudaStream_t)stream;

@@ -183,6 +183,7 @@ bool paged_append(int64_t cache, int64_t device, const at::Tensor &key, const at
                   const at::Tensor &status) {
   const auto *c = reinterpret_cast<const mxq_paged_cache *>(cache);
   if (!on(key, device) || !on(value, device) || !float_type(key) || value.scalar_type() != key.scalar_type() ||
+      (at::GradMode::is_enabled() && (key.requires_grad() || value.requires_grad())) ||
       !plain_table(table, lengths, device) || key.dim() != 4 || key.sizes() != value.sizes() ||
       key.size(0) != table.size(0) || key.size(1) != c->heads || key.size(3) != c->head_dim || key.numel() == 0 ||
       !plain_rows(key) || !plain_rows(value))

@@ -151,6 +151,7 @@ class PagedKVCache:
         self._desc = _lib.PagedCache(ptr(key), ptr(value), ptr(key_scales), ptr(value_scales), self.num_pages, code, bits,
                                      self.num_kv_heads, dim, self.page_size, 0)
         self._addr = ctypes.addressof(self._desc)
+        _status(self.device)  # made here, not during a capture
 
     def _log2_tab(self, dtype: torch.dtype):
         if self._code == _lib.CACHE_BF16:
@@ -210,7 +211,8 @@ def paged_kv_append(cache: PagedKVCache, key: Tensor, value: Tensor, page_table:
     """Quantize key / value [batch, num_kv_heads, tokens, head_dim] (fp32 or bf16, any strides) into the pages: token t of
     sequence b goes to slot lengths[b] + t.  `counts` (int32 [batch]): only the first counts[b] tokens of sequence b exist
     (a padded batch).  Codes and shared exponents are those of `mxfp_quantizer` / `mxint_quantizer` along head_dim.
-    `lengths` is not changed: add the new tokens to it once every layer has them.
+    `lengths` is not changed: add the new tokens to it once every layer has them.  The pages that are written belong to one
+    sequence of the batch each.
 
     `positions` (int32 [batch, num_kv_heads, width]) is the record of token positions that `paged_kv_evict` keeps: the
     entries of the new slots become next_position[b] + t (int32 [batch]; default: lengths[b] + t)."""
@@ -223,6 +225,8 @@ def paged_kv_append(cache: PagedKVCache, key: Tensor, value: Tensor, page_table:
     if key.dtype not in _DT or value.dtype != key.dtype:
         raise NotImplementedError(f"paged_kv_append: dtypes {key.dtype} / {value.dtype} are not supported "
                                   "(float32 and bfloat16 are, the same for both)")
+    if torch.is_grad_enabled() and (key.requires_grad or value.requires_grad):
+        raise NotImplementedError("a paged cache has no backward pass: append to it under torch.no_grad()")
     batch = _check_table(cache, page_table, lengths)
     if key.dim() != 4 or key.shape != value.shape or key.shape[0] != batch or key.shape[1] != cache.num_kv_heads \
             or key.shape[3] != cache.head_dim:
@@ -354,7 +358,8 @@ def paged_kv_evict(cache: PagedKVCache, page_table: Tensor, lengths: Tensor, wei
     nothing has been evicted yet and slot i holds position i; next_position then is `lengths`.
 
     Returns (lengths, weights, positions) of the shrunken sequences as new tensors; entries behind the new length are 0
-    and -1.  The pages behind ceil(length / page_size) are free."""
+    and -1.  The pages behind ceil(length / page_size) are free.  Rows move inside a sequence's pages: none of them may be
+    shared with another sequence."""
     ext = _binding()
     if ext and (got := ext.paged_evict(cache._addr, cache._index, page_table, lengths, weights, keep, recent, positions,
                                        next_position, _status(cache.device))) is not None:
@@ -407,7 +412,8 @@ class PagedKVState:
 
     counts (int32 [batch] or None): how many of the forward's tokens each sequence has (a right-padded batch); set it before
     the forward, `advance` uses it and clears it.  max_length is the host's bound on the lengths: dense tensors are that
-    long (plus the new tokens)."""
+    long (plus the new tokens).  `lengths` and `next_position` are updated in place.  There is no backward pass: run the
+    model under torch.no_grad()."""
 
     def __init__(self, caches: list[PagedKVCache], page_table: Tensor, lengths: Tensor | None = None, max_length: int = 0,
                  track: bool = False):
@@ -477,9 +483,10 @@ class PagedKVState:
 
     def advance(self, tokens: int) -> None:
         """The forward's tokens are now cached in every layer."""
-        after = self.lengths_after(tokens)
+        self.lengths_after(tokens)  # checks the room
         new = tokens if self.counts is None else self.counts
-        self.lengths, self.next_position = after, self.next_position + new
+        self.lengths.add_(new)
+        self.next_position.add_(new)
         self.max_length += tokens
         self.counts = self._after = None
 
@@ -490,4 +497,5 @@ class PagedKVState:
         for i, cache in enumerate(self.caches):
             lengths, self.weights[i], self.positions[i] = paged_kv_evict(
                 cache, self.page_table, self.lengths, self.weights[i], keep, recent, self.positions[i], self.next_position)
-        self.lengths, self.max_length, self._after = lengths, min(self.max_length, keep), None
+        self.lengths.copy_(lengths)
+        self.max_length, self._after = min(self.max_length, keep), None

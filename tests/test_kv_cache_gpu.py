@@ -205,7 +205,8 @@ def test_attention_against_64_bits(name, dtype, dim, page, heads, group):
     check_attention(out[:, :, 0], q[:, :, 0], k, v, lens, dim ** -0.5)
 
 
-@pytest.mark.parametrize("name,group,dtype", [("e4m3", 4, torch.bfloat16), ("int8", 1, torch.float32), ("none", 8, torch.bfloat16),
+@pytest.mark.parametrize("name,group,dtype", [("e4m3", 4, torch.bfloat16), ("e5m2", 2, torch.bfloat16), ("int8", 19, torch.bfloat16),
+                                              ("e4m3", 11, torch.float32), ("int8", 1, torch.float32), ("none", 8, torch.bfloat16),
                                               ("e2m1", 12, torch.bfloat16)])
 def test_attention_split_over_the_length(name, group, dtype):
     """Lengths that end anywhere in the split, a table that is much wider than most sequences, accumulated weights."""
@@ -665,6 +666,8 @@ def test_refusals():
             mb.paged_kv_append(cache, bad[:, :2], bad[:, :2], table, lens)
     with pytest.raises(NotImplementedError):
         mb.paged_kv_append(cache, kv, kv.float(), table, lens)
+    with pytest.raises(NotImplementedError):
+        mb.paged_kv_append(cache, kv.float().requires_grad_(), kv.float(), table, lens)
     for bad in (q[:, :3], q[:1], q[..., :32], q.expand(2, 4, 2, 64), q[:, :0]):
         with pytest.raises(ValueError):
             mb.paged_attention(cache, bad, table, lens)
