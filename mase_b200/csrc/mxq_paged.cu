@@ -616,7 +616,8 @@ static unsigned grid_x(int64_t need, int64_t yz, int per_sm) {
   int64_t most = ((int64_t)gemm::sm_count() * per_sm + yz - 1) / yz;
   if (most < 1) most = 1;
   if (need < 1) need = 1;
-  return (unsigned)(need < most ? need : most);
+  const int64_t rounds = (need + most - 1) / most;  // of every CTA, the same for all
+  return (unsigned)((need + rounds - 1) / rounds);
 }
 
 }  // namespace paged
@@ -659,7 +660,7 @@ int mxq_paged_append(const mxq_paged_cache *cache, const void *key, const void *
   const Table t{page_table, table_stride, table_width};
   const int dim = cache->head_dim;
   const int64_t yz = (int64_t)c.heads * 2 * batch;
-  const dim3 grid(grid_x((tokens * (dim / 16) + 2 * kThreads - 1) / (2 * kThreads), yz, 4), c.heads * 2, (unsigned)batch);
+  const dim3 grid(grid_x((tokens * (dim / 16) + 2 * kThreads - 1) / (2 * kThreads), yz, 8), c.heads * 2, (unsigned)batch);
   cudaStream_t st = (cudaStream_t)stream;
 #define CALL(f)                                                                                                            \
   if (cache->format == f)                                                                                                  \
@@ -686,7 +687,7 @@ int mxq_paged_gather(const mxq_paged_cache *cache, void *key, void *value, int d
   const Table t{page_table, table_stride, table_width};
   const int dim = cache->head_dim;
   const int64_t yz = (int64_t)c.heads * 2 * batch;
-  const dim3 grid(grid_x((max_tokens * (dim / 16) + kThreads - 1) / kThreads, yz, 8), c.heads * 2, (unsigned)batch);
+  const dim3 grid(grid_x((max_tokens * (dim / 16) + kThreads - 1) / kThreads, yz, 16), c.heads * 2, (unsigned)batch);
   cudaStream_t st = (cudaStream_t)stream;
 #define CALL(f)                                                                                                             \
   if (cache->format == f)                                                                                                   \
