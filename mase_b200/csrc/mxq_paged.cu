@@ -453,6 +453,7 @@ evict_select_kernel(const Cache c, int64_t table_tokens, const EvictArgs a) {
     int cnt[kOwn] = {}, s = 0;
     const int low = bins - kOwn - kOwn * tid;
     if (low >= 0)
+#pragma unroll 4
       for (int r = 0; r < size; ++r) {
         const int4 h = *reinterpret_cast<const int4 *>(size > 1 ? cluster.map_shared_rank(&hist[pass][low], r) : &hist[pass][low]);
         cnt[0] += h.w, cnt[1] += h.z, cnt[2] += h.y, cnt[3] += h.x;
@@ -494,12 +495,8 @@ evict_select_kernel(const Cache c, int64_t table_tokens, const EvictArgs a) {
   }
   more_low = warp_total(more_low), more_high = warp_total(more_high);
   tie_low = warp_total(tie_low), tie_high = warp_total(tie_high);
-  // sum over the CTAs before this one of one of their counts
-  auto before = [&](int which) {
-    int sum = 0;
-    for (int r = 0; r < rank; ++r) sum += *cluster.map_shared_rank(&counts[which], r);
-    return sum;
-  };
+  // sum over the CTAs before this one of one of their counts, by a whole warp
+  auto before = [&](int which) { return warp_total(lane < rank ? *cluster.map_shared_rank(&counts[which], lane) : 0); };
   int total;
   int seen = scan_warps(tie_low + tie_high, scratch, total);  // ties before the warp's part
   if (size > 1) {
@@ -515,8 +512,9 @@ evict_select_kernel(const Cache c, int64_t table_tokens, const EvictArgs a) {
   if (size > 1) {
     if (tid == 0) counts[1] = n_holes, counts[2] = n_movers;
     cluster.sync();
-    hole_at += before(1), mover_at += before(2);
-    if (rank == size - 1 && tid == 0) a.moves[row] = before(1) + n_holes;
+    const int holes_before = before(1);
+    hole_at += holes_before, mover_at += before(2);
+    if (rank == size - 1 && tid == 0) a.moves[row] = holes_before + n_holes;
   } else if (tid == 0) {
     a.moves[row] = n_holes;
   }
@@ -557,7 +555,7 @@ evict_select_kernel(const Cache c, int64_t table_tokens, const EvictArgs a) {
 // A warp takes `per_warp` moves at a time (up to 32): each lane looks one of them up (slots, pages) and moves its statistics, then the warp
 // copies the key and value rows of all of them, 16 bytes a lane with four copies in flight.  Sources lie at or above
 // `keep`, destinations below it, so moves never overlap.
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, 6)
 evict_move_kernel(const Cache c, const Table table, const EvictArgs a, int row_bytes_log2, int scale_bytes, int per_warp) {
   wait_for_previous();
   let_next_start();
@@ -613,7 +611,7 @@ evict_move_kernel(const Cache c, const Table table, const EvictArgs a, int row_b
 
 // CTAs along x so that the whole grid holds about `per_sm` CTAs per SM, and no more than the work needs.
 static unsigned grid_x(int64_t need, int64_t yz, int per_sm) {
-  int64_t most = ((int64_t)gemm::sm_count() * per_sm + yz - 1) / yz;
+  int64_t most = (int64_t)gemm::sm_count() * per_sm / yz;
   if (most < 1) most = 1;
   if (need < 1) need = 1;
   const int64_t rounds = (need + most - 1) / most;  // of every CTA, the same for all
@@ -756,10 +754,10 @@ int mxq_paged_evict(const mxq_paged_cache *cache, int64_t batch, const int32_t *
   const int row_bytes = row_bytes_of(cache->format, cache->head_dim);
   const int scale_bytes = cache->format == MXQ_CACHE_BF16 ? 0 : cache->head_dim / 32;
   // moves a warp looks up at once: 32, or fewer so that there is work for four warps on every SM
-  int per_warp = 32;
+  int per_warp = 8;
   while (per_warp > 4 && rows * most < (int64_t)gemm::sm_count() * 4 * per_warp) per_warp /= 2;
   const int64_t per_cta = kThreads / 32 * per_warp;
-  const dim3 grid(grid_x((most + per_cta - 1) / per_cta, rows, 8), (unsigned)c.heads, (unsigned)batch);
+  const dim3 grid(grid_x((most + per_cta - 1) / per_cta, rows, 6), (unsigned)c.heads, (unsigned)batch);
   return launch_chained(evict_move_kernel, grid, kThreads, 0, st, 1, c, t, a, log2_of(row_bytes), scale_bytes, per_warp);
 }
 

@@ -781,7 +781,6 @@ finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
   const int warps = gridDim.x * (kFinishThreads / 32), g_first = blockIdx.x * (kFinishThreads / 32) + warp;
   locate(min(g_first, a.group - 1), first, last, late);
   wait_for_previous();
-  let_next_start();
 
   // One warp for a head.  A part is dim / 4 vectors: lanes beyond that take further parts, to be added up at the end.
   const int vecs = dim >> 2;
