@@ -6,15 +6,21 @@
 // 16-row operand and the query heads of one key/value head are the 8 columns:
 //   S^T[token, head] = K[token, d] Q^T[d, head]          rows = tokens, accumulated over head_dim
 //   O^T[d, head]    += V^T[d, token] P^T[token, head]    rows = d, accumulated over the tokens of all tiles
-// The order of the summed index of a product is free, and so is the order of the rows of O^T, so every lane loads its
-// operands straight from the pages in pieces of up to 16 contiguous bytes (four lanes share a key row, eight lanes a value
-// row) and no transposition of the cache goes through shared memory; Q^T and the output follow the same permutation.
+// The order of the summed index of a product is free, and so is the order of the rows of O^T, so a lane's operands are
+// pieces of up to 16 contiguous bytes of a row (four lanes share a key row, eight lanes a value row) and nothing is
+// transposed in memory; Q^T and the output follow the same permutation.  Tiles reach shared memory by asynchronous copies
+// in address order: with every lane copying its own operand pieces the same bytes arrived at 3.9 TB/s instead of 6.7.
 //
 // Codes become bf16 in registers: sign, exponent and fraction fields are moved to the bf16 positions with masks and
 // shifts and the result is multiplied by one power of two (block scale times the difference of the exponent biases).
 // Every value of every format has at most 8 significant bits, so this is exact, subnormal codes included.  bf16 queries
 // are exact operands too; fp32 queries are split into three bf16 terms.  Probabilities are fp32 and enter the second
 // product as two (fp32 queries: three) bf16 terms, 16 (24) significant bits; scores, maxima, sums and O^T are fp32.
+//
+// Bound: HBM in principle (2 g multiply-adds per cached byte of a group of g query heads), in practice the instructions
+// that make bf16 of codes: about 570 a tile of 16 x 128 one-byte codes, 300 of them conversions; issue slots 63 % and the
+// logic unit 55 % busy.  Measured: 2 x 131072 tokens, 8 heads of 128, MXINT8: 106 us, 4.6 TB/s; 32 sequences of up to 8192,
+// E4M3: 69 us, 4.1 TB/s; bf16 pages, 16 x 2049 x 32 heads of 64: 37 us, 5.0 TB/s; copies alone reach 5.8 TB/s.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -33,7 +39,8 @@ namespace paged {
 constexpr int kWarps = 4;
 constexpr int kTile = 16;                // cached tokens of a warp's tile
 constexpr int kUnit = kWarps * kTile;    // tokens that a CTA takes at a time: the grain of the split
-constexpr int kRowCost = 2;            // units that a row counts for beyond its tokens
+constexpr int kRowCost = 2;              // units that a row counts for beyond its tokens: 1 / 2 / 4 made 84 / 78 / 80 us of
+                                         // 32 ragged sequences of up to 8192 tokens
 constexpr int kFinishThreads = 128;
 
 struct AttnArgs {
@@ -131,7 +138,7 @@ struct Shape {
   static __host__ __device__ constexpr int value_turn(int i) {
     return kRow == 128 ? ((i >> 8) & 3) << 5 : (kRow == 256 ? ((i >> 9) & 3) << 5 : (kRow == 512 ? ((i >> 10) & 3) << 5 : 0));
   }
-  static constexpr int kStages = kRow <= 64 ? 4 : 2;
+  static constexpr int kStages = kRow <= 64 ? 4 : 2;  // three for rows of 128 bytes: 109 us against 107 (2 x 131072 MXINT8)
 };
 // element (0 .. D-1) that half `half` of pair i of key word w of piece c of lane t holds
 template <int kFormat, int D>
@@ -235,11 +242,13 @@ struct Worker {
     const float c_hi = a.c_hi, c_lo = a.c_lo;
     const int t = lane & 3, r = lane >> 2;
     const int offset = raw_offset<kFormat>(bits);
-    float s[NT][4], s_odd[NT][4];  // two chains of products: even and odd steps
+    // Two chains of products, even and odd steps, and for fp32 queries one of their lower terms: the tensor cores cut off what
+    // lies below the last bit of the larger summand, which the small terms would only multiply.
+    float s[NT][4], s_odd[NT][4], s_low[NT][4];
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[n][i] = s_odd[n][i] = 0.f;
+      for (int i = 0; i < 4; ++i) s[n][i] = s_odd[n][i] = s_low[n][i] = 0.f;
 #pragma unroll
     for (int c = 0; c < S::kKeyPieces; ++c) {
       uint32_t pairs[2][S::kKeyWords * S::kPairs];
@@ -264,14 +273,14 @@ struct Worker {
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int z = kTerms - 1; z >= 0; --z)
-            mma((c * kStepsHere + k) & 1 ? s_odd[n] : s[n], rows, q[z][c * kStepsHere + k][n][0],
+            mma(z > 0 ? s_low[n] : ((c * kStepsHere + k) & 1 ? s_odd[n] : s[n]), rows, q[z][c * kStepsHere + k][n][0],
                 q[z][c * kStepsHere + k][n][1]);
       }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[n][i] += s_odd[n][i];
+      for (int i = 0; i < 4; ++i) s[n][i] += kTerms > 1 ? s_odd[n][i] + s_low[n][i] : s_odd[n][i];
     // rows: tokens r (entries 0, 1) and r + 8 (2, 3); columns: heads 2t, 2t + 1
     float x[NT][4], top = kLowest;
 #pragma unroll
@@ -387,9 +396,18 @@ struct Worker {
           const int j = (c * S::kValElems + w * kPerWord + k) / 2;
           const uint32_t rows[4] = {e[0][k], e[0][k + 1], e[1][k], e[1][k + 1]};
 #pragma unroll
-          for (int n = 0; n < NT; ++n)
+          for (int n = 0; n < NT; ++n) {
+            if constexpr (Elem<T>::kBf16) {
 #pragma unroll
-            for (int z = kPTerms - 1; z >= 0; --z) mma(o[j][n], rows, pb[z][n][0], pb[z][n][1]);
+              for (int z = kPTerms - 1; z >= 0; --z) mma(o[j][n], rows, pb[z][n][0], pb[z][n][1]);
+            } else {  // a tile's sum by itself, added with rounding: no cut-off at the size of O^T, tile after tile
+              float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int z = kPTerms - 1; z >= 0; --z) mma(part, rows, pb[z][n][0], pb[z][n][1]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[j][n][i] += part[i];
+            }
+          }
         }
       }
     }
@@ -486,6 +504,7 @@ __device__ __forceinline__ bool any_rare(uint32_t w, int bits) {
   }
 }
 
+// Three CTAs per SM where the registers would allow two: 107 us on 2 x 131072 MXINT8 tokens; four spill, 114 us.
 template <typename T, int kFormat, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, Elem<T>::kBf16 && D == 128 && NT == 1 ? 3 : 1)
 attention_kernel(const Cache c, const Table table, const AttnArgs a) {
@@ -835,7 +854,7 @@ finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
 }
 
 // Query heads in tiles of 8, or of 16 for bf16 queries of more than 8 heads a group and head_dim <= 128 (larger ones do
-// not fit the registers).
+// not fit the registers): 16 heads a group over 8 x 8192 E4M3 tokens of 8 heads of 128 take 52 us in one tile, 64 us in two.
 static int tiles_per_row(int dtype, int dim, int64_t group) { return dtype == MXQ_BF16 && group > 8 && dim <= 128 ? 2 : 1; }
 constexpr int kMostPerSm = 8;  // CTAs of the attention kernel on one SM, at most
 

@@ -411,12 +411,12 @@ class PagedKVState:
     cached rows back as dense tensors.
 
     counts (int32 [batch] or None): how many of the forward's tokens each sequence has (a right-padded batch); set it before
-    the forward, `advance` uses it and clears it.  max_length is the host's bound on the lengths: dense tensors are that
-    long (plus the new tokens).  `lengths` and `next_position` are updated in place.  There is no backward pass: run the
+    the forward, `advance` uses it and clears it.  max_length is the host's bound on the lengths (default: their
+    maximum now): dense tensors are that long, plus the new tokens.  `lengths` and `next_position` are updated in place.  There is no backward pass: run the
     model under torch.no_grad()."""
 
-    def __init__(self, caches: list[PagedKVCache], page_table: Tensor, lengths: Tensor | None = None, max_length: int = 0,
-                 track: bool = False):
+    def __init__(self, caches: list[PagedKVCache], page_table: Tensor, lengths: Tensor | None = None,
+                 max_length: int | None = None, track: bool = False):
         if not caches:
             raise ValueError("PagedKVState needs the cache of at least one layer")
         first = caches[0]
@@ -425,7 +425,9 @@ class PagedKVState:
                 raise ValueError("the layers' caches have the same heads and page size and are on one device")
         self.caches, self.page_table = list(caches), page_table
         if lengths is None:
-            lengths = torch.zeros(page_table.shape[0], dtype=torch.int32, device=first.device)
+            lengths, max_length = torch.zeros(page_table.shape[0], dtype=torch.int32, device=first.device), max_length or 0
+        elif max_length is None:
+            max_length = int(lengths.max()) if lengths.numel() else 0
         batch = _check_table(first, page_table, lengths)
         self.lengths, self.max_length, self.counts = lengths, max_length, None
         self.capacity = page_table.shape[1] * first.page_size
@@ -436,7 +438,7 @@ class PagedKVState:
             slots = torch.arange(self.capacity, dtype=torch.int32, device=first.device).expand(shape)
             self.weights = [torch.zeros(shape, dtype=torch.float32, device=first.device) for _ in caches]
             self.positions = [slots.contiguous() for _ in caches]
-        self._after = None  # (tokens, lengths after the forward that is under way)
+        self._after = None  # lengths after the forward that is under way, and what they were made from
 
     def check_format(self, layer_idx: int, fmt: str | None, config: dict | None) -> None:
         """Raises unless the layer's cache has the format that a block's `kv_cache` entry asks for."""
@@ -445,10 +447,12 @@ class PagedKVState:
             raise ValueError(f"layer {layer_idx}: the block's kv_cache configuration is not the format of its paged cache")
 
     def lengths_after(self, tokens: int) -> Tensor:
-        if self._after is None or self._after[0] != tokens:
-            if self.max_length + tokens > self.capacity:
-                raise ValueError(f"{self.max_length} + {tokens} tokens do not fit a page table of {self.capacity}")
-            self._after = (tokens, self.lengths + (tokens if self.counts is None else self.counts))
+        if self.max_length + tokens > self.capacity:
+            raise ValueError(f"{self.max_length} + {tokens} tokens do not fit a page table of {self.capacity}")
+        c = self.counts
+        key = (tokens, self.lengths._version, None if c is None else (id(c), c._version))
+        if self._after is None or self._after[0] != key:  # once for all layers
+            self._after = (key, self.lengths + (tokens if c is None else c), c)
         return self._after[1]
 
     def append(self, key: Tensor, value: Tensor, layer_idx: int) -> None:

@@ -232,6 +232,23 @@ def test_attention_split_over_the_length(name, group, dtype):
     assert_bits_equal(mb.paged_attention(cache, q.to(DEV), table, i32(lens)), out, "second call")
 
 
+@pytest.mark.parametrize("batch,longest,group", [(300, 40, 2), (70, 700, 1), (1000, 3, 16)])
+def test_many_short_sequences(batch, longest, group):
+    """More sequences than one warp looks at, rows that begin and end inside every CTA, rows of single tokens."""
+    g = torch.Generator().manual_seed(batch)
+    lens = torch.randint(0, longest + 1, (batch,), generator=g).tolist()
+    cache, table = make_cache("int8", 3, 32, 16, lens, seed=6)
+    k, v = fill(cache, table, lens, "int8", seed=23)
+    q = rows(batch, 3 * group, 32, seed=24, dtype=torch.bfloat16)
+    acc = torch.zeros(batch, 3, longest, device=DEV)
+    out = mb.paged_attention(cache, q.to(DEV), table, i32(lens), weights=acc)
+    gemm.check_status()
+    w, bound = check_attention(out, q, k, v, lens, 32 ** -0.5)
+    tol = w * weight_error(bound, 32).view(batch, 3, -1).amax(-1, keepdim=True) + 2.0 ** -23
+    most = w.shape[2]
+    assert bool(((acc.double().cpu()[:, :, :most] - w).abs() <= tol).all()) and bool((acc[:, :, most:] == 0).all())
+
+
 @pytest.mark.parametrize("name", ["e4m3", "e5m2", "e2m1", "int8", "none"])
 @pytest.mark.parametrize("scale", [2.0 ** 40, 2.0 ** 100, 2.0 ** -60, 2.0 ** -100])
 def test_attention_at_the_ends_of_the_range(name, scale):
@@ -454,6 +471,83 @@ def test_prompt_steps_and_eviction_together(name):
         for b in range(n):
             for h in range(heads):
                 assert torch.allclose(weights[b, h, : len(acc[b][h])].double().cpu(), acc[b][h], rtol=1e-4, atol=1e-5)
+    gemm.check_status()
+
+
+def test_steps_without_a_pause():
+    """Kernels are set up while their predecessors drain: every call still sees what the calls before it wrote, torch's
+    in-place additions to the lengths among them."""
+    n, heads, dim, steps = 3, 2, 64, 60
+    cache, table = make_cache("e4m3", heads, dim, 16, [steps + 5] * n, seed=15)
+    start = [0, 5, 2]
+    k0, v0 = fill(cache, table, start, "e4m3", seed=16)
+    new = [[rows(n, heads, 1, dim, seed=300 + 2 * i + s, dtype=torch.bfloat16) for s in (0, 1)] for i in range(steps)]
+    qs = [rows(n, heads * 4, dim, seed=500 + i, dtype=torch.bfloat16) for i in range(steps)]
+    on_gpu = [[t.to(DEV) for t in pair] + [q.to(DEV)] for pair, q in zip(new, qs)]
+    lengths, outs = i32(start), []
+    torch.cuda.synchronize()
+    for key, value, q in on_gpu:
+        mb.paged_kv_append(cache, key, value, table, lengths)
+        lengths.add_(1)
+        outs.append(mb.paged_attention(cache, q, table, lengths))
+    gemm.check_status()
+    dense = [[torch.cat([x[b, :, : start[b]]] + [fake(p[s][b], "e4m3").double() for p in new], 1) for b in range(n)]
+             for s, x in ((0, k0), (1, v0))]
+    for i in range(steps):
+        for b in range(n):
+            m = start[b] + i + 1
+            check_attention(outs[i][b : b + 1], qs[i][b : b + 1], dense[0][b][None, :, :m], dense[1][b][None, :, :m], [m], 0.125)
+
+
+def test_two_streams_at_once():
+    """The same cache read by calls on two streams at the same time: workspaces are their own."""
+    lens = [5000, 300]
+    cache, table = make_cache("int8", 4, 128, 64, lens, seed=17)
+    k, v = fill(cache, table, lens, "int8", seed=18)
+    qs = [rows(2, 16, 128, seed=19 + i, dtype=torch.bfloat16) for i in range(2)]
+    on_gpu, lengths = [q.to(DEV) for q in qs], i32(lens)
+    alone = [mb.paged_attention(cache, q, table, lengths) for q in on_gpu]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(mb.paged_attention(cache, on_gpu[i], table, lengths))
+    torch.cuda.synchronize()
+    gemm.check_status()
+    for i in range(2):
+        check_attention(alone[i], qs[i], k, v, lens, 128 ** -0.5)
+        for out in got[i]:
+            assert torch.equal(out, alone[i])
+
+
+def test_captured_eviction():
+    """Eviction and read-back in a graph follow the weights and lengths of each replay."""
+    cache, table = make_cache("e4m3", 2, 64, 16, [100, 90], seed=25)
+    fill(cache, table, [100, 90], "e4m3", seed=26)
+    kept = [t.clone() for t in (cache.key, cache.value, cache.key_scales, cache.value_scales)]
+    w, lengths = torch.rand(2, 2, 112, device=DEV), i32([100, 90])
+    mb.paged_kv_evict(cache, table, lengths, w, 30, 5)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        lens, new_w, pos = mb.paged_kv_evict(cache, table, lengths, w, 30, 5)
+        k, _ = mb.paged_kv_gather(cache, table, lens, 30)
+    for seed, n in ((1, [100, 90]), (2, [64, 20]), (3, [31, 90])):
+        results = []
+        for how in (g.replay, None):
+            for t, u in zip((cache.key, cache.value, cache.key_scales, cache.value_scales), kept):
+                t.copy_(u)
+            w.copy_(torch.rand(2, 2, 112, generator=torch.Generator().manual_seed(seed)))
+            lengths.copy_(i32(n))
+            if how is not None:
+                how()
+                results.append([t.clone() for t in (lens, new_w, pos, k)])
+            else:
+                a = mb.paged_kv_evict(cache, table, lengths, w, 30, 5)
+                results.append([*a, mb.paged_kv_gather(cache, table, a[0], 30)[0]])
+        for x, y in zip(*results):
+            assert torch.equal(x, y)
     gemm.check_status()
 
 
