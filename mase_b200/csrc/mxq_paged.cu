@@ -299,9 +299,9 @@ gather_kernel(const Cache c, const Table table, const int32_t *lengths, T *key, 
 // Selection: a cluster of 1 to 8 CTAs per (sequence, head), each with a contiguous part of the slots.  The weights become
 // 32-bit keys whose unsigned order is the order of preference; three passes over 11 + 11 + 10 bits of the keys (a
 // histogram in each CTA's shared memory, added up over the cluster) find the key of the last token kept, and every warp
-// then walks a contiguous part of the slots, four neighbours a lane, so that ranks follow the slot order.  Keys live in shared memory
-// when they fit and are read again from L2 otherwise.  Bound by the chain of barriers and scans, not by its 16 bytes a slot:
-// 64 rows of 16384 slots take 20 us, 8 rows of 1500 slots 6 to 9; with the moves behind it 69 and 11 us.
+// then walks a contiguous part of the slots, four neighbours a lane, so that ranks follow the slot order.  Keys live in
+// shared memory when they fit and are read again from L2 otherwise.  Bound by the chain of barriers and scans, not by its
+// 16 bytes a slot: 64 rows of 16384 slots take 20 us, 8 rows of 1500 slots 6 to 9; with the moves behind it 69 and 11 us.
 constexpr int kSelectThreads = 512;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kBins = 2048;
@@ -556,9 +556,9 @@ evict_select_kernel(const Cache c, int64_t table_tokens, const EvictArgs a) {
   if (size > 1) cluster.sync();  // no CTA leaves while another may still read its counts
 }
 
-// A warp takes `per_warp` moves at a time (up to 32): each lane looks one of them up (slots, pages) and moves its statistics, then the warp
-// copies the key and value rows of all of them, 16 bytes a lane with four copies in flight (with eight the whole eviction
-// takes 105 us instead of 76).  Sources lie at or above `keep`, destinations below it, so moves never overlap.  Bound by
+// A warp takes `per_warp` moves at a time (up to 32): each lane looks one of them up (slots, pages) and moves its
+// statistics, then the warp copies the key and value rows of all of them, 16 bytes a lane with four copies in flight (with
+// eight the whole eviction takes 105 us instead of 76).  Sources lie at or above `keep`, destinations below it, so moves never overlap.  Bound by
 // HBM and the latency of rows of 256 bytes in random places: 230,000 rows of 512 bytes in and out in about 45 us.
 __global__ void __launch_bounds__(kThreads, 6)
 evict_move_kernel(const Cache c, const Table table, const EvictArgs a, int row_bytes_log2, int scale_bytes, int per_warp) {
@@ -709,7 +709,7 @@ static int64_t max_moves_of(int64_t width, int64_t keep) {
 }
 
 int64_t mxq_paged_evict_workspace_bytes(const mxq_paged_cache *cache, int64_t batch, int64_t width, int64_t keep) {
-  if (!cache || batch < 0 || width < 0 || keep < 1) return MXQ_ERR_SHAPE;
+  if (!cache || batch < 0 || width < 1 || keep < 1) return MXQ_ERR_SHAPE;
   return batch * cache->heads * (2 * max_moves_of(width, keep) + 1) * 4;
 }
 
@@ -721,9 +721,9 @@ int mxq_paged_evict(const mxq_paged_cache *cache, int64_t batch, const int32_t *
   Cache c;
   int rc = read_cache(cache, c);
   if (rc != MXQ_OK) return rc;
-  if (batch < 0 || width < 0 || width > INT32_MAX || keep < 1 || keep > INT32_MAX || recent < 0 || recent > keep)
+  if (batch < 0 || width < 1 || width > INT32_MAX || keep < 1 || keep > INT32_MAX || recent < 0 || recent > keep)
     return MXQ_ERR_SHAPE;
-  if (batch == 0 || width == 0) return MXQ_OK;
+  if (batch == 0) return MXQ_OK;
   if ((rc = read_table(page_table, table_width, table_stride, batch, c.page_log2)) != MXQ_OK) return rc;
   if (!lengths || !weights || !new_lengths || !new_weights || !new_positions || !workspace) return MXQ_ERR_NULL;
   if (!aligned(workspace, 16)) return MXQ_ERR_ALIGN;

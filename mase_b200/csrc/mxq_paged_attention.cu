@@ -18,8 +18,8 @@
 // product as two (fp32 queries: three) bf16 terms, 16 (24) significant bits; scores, maxima, sums and O^T are fp32.
 //
 // Bound: HBM in principle (2 g multiply-adds per cached byte of a group of g query heads), in practice the instructions
-// that make bf16 of codes: about 570 a tile of 16 x 128 one-byte codes, 300 of them conversions; issue slots 63 % and the
-// logic unit 55 % busy.  Measured: 2 x 131072 tokens, 8 heads of 128, MXINT8: 106 us, 4.6 TB/s; 32 sequences of up to 8192,
+// that make bf16 of codes: 550 to 600 a tile of 16 x 128 one-byte codes, about 300 of them conversions; issue slots 63 % and the
+// logic unit 55 % busy.  Measured: 2 x 131072 tokens, 8 heads of 128, MXINT8: 107 us, 4.6 TB/s; 32 sequences of up to 8192,
 // E4M3: 69 us, 4.1 TB/s; bf16 pages, 16 x 2049 x 32 heads of 64: 37 us, 5.0 TB/s; copies alone reach 5.8 TB/s.
 
 #include <cuda_bf16.h>
@@ -983,7 +983,7 @@ int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, 
   if (weights && weights_width < 1) return MXQ_ERR_SHAPE;
   const int dim = cache->head_dim;
   const int64_t tokens = table_width << c.page_log2;
-  if (cache->pages * ((int64_t)c.heads << c.page_log2) * row_bytes_of(cache->format, dim) > MXQ_CACHE_SIDE_BYTES)
+  if (c.pages > MXQ_CACHE_SIDE_BYTES / (((int64_t)c.heads << c.page_log2) * row_bytes_of(cache->format, dim)))
     return MXQ_ERR_SHAPE;  // tiles are addressed by 32-bit multiples of 16 bytes
   const int nt = tiles_per_row(dtype, dim, group);
   int64_t most_ctas;

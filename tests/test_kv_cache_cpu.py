@@ -82,6 +82,9 @@ def test_bad_arguments_are_refused(library):
     assert attention(q=None) == -5 and attention(lengths=None) == -5 and attention(table=None) == -5
     assert attention(weights=256, ww=0) == -2
     assert attention(width=64, ws=None) == -5 and attention(width=64, ws=264) == -4 and attention(width=64, n_ws=64) == -2
+    big = desc(pages=2 ** 31 - 1, heads=32767, head_dim=256, page_size=256, format=_lib.CACHE_BF16)
+    assert library.mxq_paged_attention(ctypes.addressof(big), 256, 256, 1, 1, 32767, 64, 64, 1.0, 256, 1, 1, 256, None, 0, 256,
+                                       1 << 40, None, None) == -2  # keys of more than 64 GiB
     need = library.mxq_paged_attention_workspace_bytes
     assert need(c, 1, 2, 64, 0) > 0 and need(c, 1, 2, 64, 1) > need(c, 1, 2, 64, 0) and need(c, 1, 3, 64, 0) == -2
     assert need(c, 0, 2, 64, 0) == 0
@@ -90,7 +93,7 @@ def test_bad_arguments_are_refused(library):
         return library.mxq_paged_evict(c, batch, table, 2, 2, lengths, weights, None, None, width, keep, recent, out, out, out,
                                        ws, n_ws, None, None)
 
-    assert evict(batch=0) == 0 and evict(width=0) == 0
+    assert evict(batch=0) == 0 and evict(width=0) == -2
     assert evict(keep=0) == -2 and evict(recent=5) == -2 and evict(recent=-1) == -2 and evict(n_ws=8) == -2
     assert evict(weights=None) == -5 and evict(ws=None) == -5 and evict(ws=260) == -4 and evict(table=None) == -5
     assert library.mxq_paged_evict_workspace_bytes(c, 3, 32, 4) == 3 * 2 * 9 * 4
