@@ -41,7 +41,7 @@ constexpr int kTile = 16;                // cached tokens of a warp's tile
 constexpr int kUnit = kWarps * kTile;    // tokens that a CTA takes at a time: the grain of the split
 constexpr int kRowCost = 2;              // units that a row counts for beyond its tokens: 1 / 2 / 4 made 84 / 78 / 80 us of
                                          // 32 ragged sequences of up to 8192 tokens
-constexpr int kFinishThreads = 128;
+__host__ __device__ constexpr int finish_threads(int w) { return w > 4 ? 32 * w : 128; }
 
 struct AttnArgs {
   const void *q;
@@ -754,12 +754,14 @@ attention_kernel(const Cache c, const Table table, const AttnArgs a) {
 
 // Joins the parts of the rows that CTAs share, and adds the softmax weights of every token to the caller's statistics:
 //   weights[b, head, j] += sum over the group of exp(s_j - m) / l.
-// grid: (x, heads, batch): the x CTAs' warps take the heads of the group in turn, and their threads the tokens.
+// grid: (x, heads, batch): the x CTAs take the heads of the group in turn, W warps a head, and their threads the tokens.
 // Before the wait only what the attention kernel does not write is read: its CTAs let this kernel start after their own
 // wait, so everything before it in the stream has finished.
-template <typename T>
-__global__ void __launch_bounds__(kFinishThreads)
+template <typename T, int W>
+__global__ void __launch_bounds__(finish_threads(W))
 finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
+  constexpr int kThreads = finish_threads(W), kAtOnce = kThreads / 32 / W;  // heads of the group at a time
+  __shared__ float4 sums[W > 1 ? kThreads : 1];
   extern __shared__ float2 stats[];  // [group] pairs of maximum and 1 / sum
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int head = blockIdx.y, b = blockIdx.z;
@@ -782,6 +784,7 @@ finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
   auto join = [&](int g, int first, int last, bool late) {
     if (first == last) return a.stats != nullptr ? a.stats[(int64_t)b * a.q_heads + head * a.group + g] : make_float2(0.f, 0.f);
     float top = kLowest, sum = 0.f;
+#pragma unroll 8
     for (int c = first + lane; c <= last; c += 32) {  // running maximum and sum: one pass over the parts
       const float2 p = a.part_ml[part_of(c, first, late, g)];
       const float high = fmaxf(top, p.x);
@@ -797,34 +800,50 @@ finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
   };
   int first, last;
   bool late;
-  const int warps = gridDim.x * (kFinishThreads / 32), g_first = blockIdx.x * (kFinishThreads / 32) + warp;
+  const int sub = warp % W, g_first = blockIdx.x * kAtOnce + warp / W;
   locate(min(g_first, a.group - 1), first, last, late);
   wait_for_previous();
 
-  // One warp for a head.  A part is dim / 4 vectors: lanes beyond that take further parts, to be added up at the end.
-  const int vecs = dim >> 2;
-  for (int g = g_first; g < a.group; g += warps) {
-    if (g != g_first) locate(g, first, last, late);
-    if (first == last) continue;  // finished by its CTA
-    const float2 st = join(g, first, last, late);
+  // A part is dim / 4 vectors: lanes beyond that take further parts, to be added up at the end.
+  const int vecs = dim >> 2, at_once = vecs < 32 ? 32 / vecs : 1;
+  for (int g0 = blockIdx.x * kAtOnce; g0 < a.group; g0 += gridDim.x * kAtOnce) {
+    const int g = g0 + warp / W;
+    const bool there = g < a.group;
+    if (there && g != g_first) locate(g, first, last, late);
+    const bool parts = there && first != last;  // otherwise finished by its CTA
+    const float2 st = parts ? join(g, first, last, late) : make_float2(0.f, 0.f);
     for (int v0 = 0; v0 < vecs; v0 += 32) {  // more than once for head_dim 256
-      const int at_once = vecs < 32 ? 32 / vecs : 1, vec = v0 + (vecs < 32 ? lane & (vecs - 1) : lane);
+      const int vec = v0 + (vecs < 32 ? lane & (vecs - 1) : lane);
       float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (parts) {
 #pragma unroll 8
-      for (int c = first + (vecs < 32 ? lane / vecs : 0); c <= last; c += at_once) {
-        const int64_t part = part_of(c, first, late, g);
-        const float f = exp2f(a.part_ml[part].x - st.x);
-        const float4 o = reinterpret_cast<const float4 *>(a.part_o + part * dim)[vec];
-        v.x += f * o.x, v.y += f * o.y, v.z += f * o.z, v.w += f * o.w;
+        for (int c = first + sub * at_once + (vecs < 32 ? lane / vecs : 0); c <= last; c += W * at_once) {
+          const int64_t part = part_of(c, first, late, g);
+          const float f = exp2f(a.part_ml[part].x - st.x);
+          const float4 o = reinterpret_cast<const float4 *>(a.part_o + part * dim)[vec];
+          v.x += f * o.x, v.y += f * o.y, v.z += f * o.z, v.w += f * o.w;
+        }
+      }
+      if constexpr (W > 1) {
+        if (v0 > 0 || g0 > blockIdx.x * kAtOnce) __syncthreads();  // the sums before have been read
+        sums[tid] = v;
+        __syncthreads();
+        if (sub == 0) {
+#pragma unroll
+          for (int k = 1; k < W; ++k) {
+            const float4 o = sums[tid + 32 * k];
+            v.x += o.x, v.y += o.y, v.z += o.z, v.w += o.w;
+          }
+        }
       }
       for (int x = 16; x >= vecs; x >>= 1) {
         v.x += __shfl_xor_sync(0xFFFFFFFFu, v.x, x), v.y += __shfl_xor_sync(0xFFFFFFFFu, v.y, x);
         v.z += __shfl_xor_sync(0xFFFFFFFFu, v.z, x), v.w += __shfl_xor_sync(0xFFFFFFFFu, v.w, x);
       }
-      const float r[4] = {v.x / st.y, v.y / st.y, v.z / st.y, v.w / st.y};
-      const float none[4] = {0.f, 0.f, 0.f, 0.f};
-      T *out = static_cast<T *>(a.out) + ((int64_t)b * a.q_heads + head * a.group + g) * dim + 4 * vec;
-      if (vecs >= 32 || lane < vecs) {
+      if (parts && sub == 0 && (vecs >= 32 || lane < vecs)) {
+        const float r[4] = {v.x / st.y, v.y / st.y, v.z / st.y, v.w / st.y};
+        const float none[4] = {0.f, 0.f, 0.f, 0.f};
+        T *out = static_cast<T *>(a.out) + ((int64_t)b * a.q_heads + head * a.group + g) * dim + 4 * vec;
         if (st.y == 0.f)
           store_vals(out, 0, none);
         else
@@ -833,7 +852,7 @@ finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
     }
   }
   if (a.weights == nullptr) return;
-  for (int g = warp; g < a.group; g += kFinishThreads / 32) {
+  for (int g = warp; g < a.group; g += kThreads / 32) {
     locate(g, first, last, late);
     const float2 st = join(g, first, last, late);
     if (lane == 0) stats[g] = make_float2(st.x, st.y == 0.f ? 0.f : 1.f / st.y);
@@ -841,7 +860,7 @@ finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
   __syncthreads();
   const float *scores = a.scores + ((int64_t)b * rows + head * a.head_tiles) * a.score_tokens * a.score_heads;
   float *weights = a.weights + ((int64_t)b * heads + head) * a.weights_width;
-  for (int j = blockIdx.x * kFinishThreads + tid; j < length; j += gridDim.x * kFinishThreads) {
+  for (int j = blockIdx.x * kThreads + tid; j < length; j += gridDim.x * kThreads) {
     float sum = 0.f;
     for (int g = 0; g < a.group; g += 2) {  // two heads of a tile lie together
       const int ht = g / tile_heads;
@@ -1016,18 +1035,28 @@ int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, 
   rc = dtype == MXQ_BF16 ? launch_attention<__nv_bfloat16>(cache->format, dim, c, t, a, nt, most_ctas, st)
                          : launch_attention<float>(cache->format, dim, c, t, a, nt, most_ctas, st);
   if (rc != MXQ_OK || (!parts && !weights)) return rc;
-  int64_t x = (group + kFinishThreads / 32 - 1) / (kFinishThreads / 32);
+  // Warps for a head: one where rows are shared by few CTAs (64 sequences, 512 rows: 77 us against 89 with four), four or
+  // sixteen where they are shared by many (one row of 40000
+  // tokens in 444 parts: 21 us with sixteen, 77 with one; 16 rows of 28 parts: 105 us with four, 108 with one).
+  const int64_t per_row = a.ctas / (batch * c.heads * a.head_tiles);
+  const int w_head = per_row >= 64 ? 16 : (per_row >= 8 ? 4 : 1), threads = finish_threads(w_head);
+  const int64_t at_once = threads / 32 / w_head;
+  int64_t x = (group + at_once - 1) / at_once;
   if (weights) {  // enough CTAs for the tokens, and no more than the GPU holds at once
-    const int64_t need = (tokens + kFinishThreads - 1) / kFinishThreads;
-    const int64_t cap = ((int64_t)gemm::sm_count() * 16 + c.heads * batch - 1) / (c.heads * batch);
+    const int64_t need = (tokens + threads - 1) / threads;
+    const int64_t cap = ((int64_t)gemm::sm_count() * (2048 / threads) + c.heads * batch - 1) / (c.heads * batch);
     const int64_t most = need < cap ? need : cap;
     x = most > x ? most : x;
   }
   const dim3 grid((unsigned)x, (unsigned)c.heads, (unsigned)batch);
   const size_t smem = weights ? group * sizeof(float2) : 0;
-  return dtype == MXQ_BF16
-             ? launch_chained(finish_kernel<__nv_bfloat16>, grid, kFinishThreads, smem, st, 1, a, c.heads, 8 * nt, dim)
-             : launch_chained(finish_kernel<float>, grid, kFinishThreads, smem, st, 1, a, c.heads, 8 * nt, dim);
+#define CALL(T)                                                                                                   \
+  return w_head == 16  ? launch_chained(finish_kernel<T, 16>, grid, threads, smem, st, 1, a, c.heads, 8 * nt, dim) \
+         : w_head == 4 ? launch_chained(finish_kernel<T, 4>, grid, threads, smem, st, 1, a, c.heads, 8 * nt, dim)  \
+                       : launch_chained(finish_kernel<T, 1>, grid, threads, smem, st, 1, a, c.heads, 8 * nt, dim);
+  if (dtype == MXQ_BF16) CALL(__nv_bfloat16)
+  CALL(float)
+#undef CALL
 }
 
 }  // extern "C"
