@@ -15,7 +15,8 @@ through the split that keeps fp32-level products; bf16 products are exact.
 
 `past_key_value` is anything with the `update` of a key/value cache, or a `mase_b200.kv_cache.PagedKVState`: then keys and
 values are quantized into pages, and a step of one new token per sequence runs on the pages themselves when softmax and
-probabilities are not quantized and no mask is given (its second return value is then None).
+probabilities are not quantized and no mask is given (its second return value is then None).  Everything else reads dense
+tensors back, in which the rows behind a sequence's own tokens are masked whatever `attention_mask` says of them.
 """
 
 from __future__ import annotations
@@ -168,6 +169,8 @@ class _AttentionMX(nn.Module):
         # only the quantized operand is known to fit tf32; the other one takes the fp32 split
         weights = self._product(query, key, exact=False)
         dropout = self.training and self.attention_dropout > 0
+        if paged is not None:  # the dense tensors are as long as the longest sequence may be
+            attention_mask = paged.hide_absent(attention_mask, input_shape[-1], key.shape[-2], weights.dtype)
         # scaling, mask, the softmax with its input quantizer and the quantizer of the probabilities: one kernel
         fused = F_mx.attention_softmax(weights, self.scaling, attention_mask,
                                        None if self.softmax_bypass else "minifloat", self.softmax_config,

@@ -473,13 +473,27 @@ class PagedKVState:
         return paged_attention(self.caches[layer_idx], query, self.page_table, self.lengths_after(1), scaling,
                                None if self.weights is None else self.weights[layer_idx])
 
+    def hide_absent(self, mask: Tensor | None, tokens: int, keys: int, dtype: torch.dtype) -> Tensor:
+        """An additive mask for the scores [batch, heads, tokens, keys] over the dense tensors of `update`: `mask` with the
+        lowest value of its type at the rows that are behind a sequence's tokens (zeros in the dense tensors, which would
+        take their share of the softmax).  A sequence without tokens keeps its first row, and gets its zeros as a result."""
+        live = self.lengths_after(tokens).clamp(min=1)[:, None, None, None]
+        absent = torch.arange(keys, device=live.device) >= live  # [batch, 1, 1, keys]
+        if mask is None:
+            mask = torch.zeros((1, 1, tokens, keys), dtype=dtype, device=live.device)
+        elif not mask.is_floating_point():
+            mask = mask.to(dtype)
+        return torch.where(absent, torch.finfo(mask.dtype).min, mask[:, :, :, :keys])
+
     def accumulate(self, probabilities: Tensor, layer_idx: int) -> None:
-        """Add dense softmax weights [batch, heads, tokens, keys] of the forward's tokens to the statistics."""
+        """Add dense softmax weights [batch, heads, tokens, keys] of the forward's tokens to the statistics of the tokens
+        that each sequence has."""
         if self.weights is None:
             return
         b, h, t, n = probabilities.shape
         heads = self.caches[layer_idx].num_kv_heads
-        p = probabilities.detach().float()
+        there = torch.arange(n, device=probabilities.device) < self.lengths_after(t)[:, None]
+        p = torch.where(there[:, None, None, :], probabilities.detach().float(), 0.0)
         if self.counts is not None:  # rows of padding count for nothing
             live = torch.arange(t, device=p.device) < self.counts[:, None]
             p = torch.where(live[:, None, :, None], p, 0.0)

@@ -1,0 +1,60 @@
+"""`PagedKVState` through the attention blocks on the GPU: ragged batches without masks, captured steps, inference mode."""
+
+import pytest
+import torch
+
+import mase_b200 as mb
+from mase_b200 import gemm
+from test_kv_cache_gpu import CONFIGS, DEV, blocks, causal, i32, rope, rows
+
+pytestmark = pytest.mark.gpu
+
+
+def make_state(name, batch, width=6, layers=1, track=True, page=16):
+    fmt, cfg = CONFIGS[name]
+    caches = [mb.PagedKVCache(batch * width + 1, 2, 32, page, fmt, cfg, DEV) for _ in range(layers)]
+    table = torch.randperm(batch * width, generator=torch.Generator().manual_seed(1)).view(batch, width).int().to(DEV)
+    return mb.PagedKVState(caches, table, track=track)
+
+
+def softmax_quantized(block, av):
+    """The block with its softmax input quantized, and its probabilities if `av`."""
+    block.softmax_bypass = False
+    block.softmax_config = {"data_in_exponent_width": 5, "data_in_frac_width": 10}
+    block.av_bypass = not av
+    return block
+
+
+@pytest.mark.parametrize("mask", [None, "zeros"])
+@pytest.mark.parametrize("name,lens,av", [("e4m3", [20, 13, 0], False), ("int8", [63, 31], True)])
+def test_dense_steps_of_a_ragged_batch_without_a_mask(name, lens, av, mask):
+    """One new token per sequence through a block that needs the dense tensors: each sequence as by itself, whatever rows
+    of zeros the others' length leaves behind it.  Both sides round scores to 11 bits (a score of magnitude up to 8 moves
+    by 2**-8, a weight by 2**-7 of itself) and, for `av`, probabilities to 8: 2e-2 of the largest output; an unmasked
+    row of zeros would take 1/64 of the weight, and there are 7 to 32 of them."""
+    layer = softmax_quantized(blocks(name, torch.float32, True, layers=1)[0], av)
+    if av:
+        layer.av_config = CONFIGS[name][1]
+    n, most = len(lens), max(lens)
+    state = make_state(name, n)
+    k, v = (rows(n, 2, most, 32, seed=s, dtype=torch.float32).to(DEV) for s in (1, 2))
+    step = rows(n, 1, 128, seed=4, dtype=torch.float32, spread=0.1).to(DEV)
+    with torch.no_grad():
+        state.counts = i32(lens)
+        state.append(k, v, 0)
+        state.advance(most)
+        m = None if mask is None else torch.zeros(1, 1, 1, most + 1, device=DEV)
+        out, p = layer(step, rope(lens, 1, n, torch.float32), m, past_key_value=state)
+        assert p.shape[-1] == most + 1
+        for b, length in enumerate(lens):
+            alone = make_state(name, 1)
+            if length:
+                alone.append(k[b : b + 1, :, :length], v[b : b + 1, :, :length], 0)
+                alone.advance(length)
+            one, p1 = layer(step[b : b + 1], rope(length, 1, 1, torch.float32), None, past_key_value=alone)
+            assert p1.shape[-1] == length + 1
+            assert float((out[b] - one[0]).abs().max() / one.abs().max()) <= 2e-2, (b, length)
+            w = state.weights[0][b]
+            assert bool((w[:, length + 1 :] == 0).all())
+            assert torch.allclose(w, alone.weights[0][0], rtol=0.1, atol=2e-2)
+    gemm.check_status()
