@@ -438,7 +438,6 @@ class PagedKVState:
             slots = torch.arange(self.capacity, dtype=torch.int32, device=first.device).expand(shape)
             self.weights = [torch.zeros(shape, dtype=torch.float32, device=first.device) for _ in caches]
             self.positions = [slots.contiguous() for _ in caches]
-        self._after = None  # lengths after the forward that is under way, and what they were made from
 
     def check_format(self, layer_idx: int, fmt: str | None, config: dict | None) -> None:
         """Raises unless the layer's cache has the format that a block's `kv_cache` entry asks for."""
@@ -446,17 +445,18 @@ class PagedKVState:
         if (c._code, c._bits) != _format_of(fmt, config):
             raise ValueError(f"layer {layer_idx}: the block's kv_cache configuration is not the format of its paged cache")
 
-    def lengths_after(self, tokens: int) -> Tensor:
+    def _check_room(self, tokens: int) -> None:
         if self.max_length + tokens > self.capacity:
             raise ValueError(f"{self.max_length} + {tokens} tokens do not fit a page table of {self.capacity}")
-        c = self.counts
-        key = (tokens, self.lengths._version, None if c is None else (id(c), c._version))
-        if self._after is None or self._after[0] != key:  # once for all layers
-            self._after = (key, self.lengths + (tokens if c is None else c), c)
-        return self._after[1]
+
+    def lengths_after(self, tokens: int) -> Tensor:
+        """The lengths once the forward's tokens are cached.  Added up by every call: a sum that is kept would not be part
+        of a captured graph, and replays of one change the lengths behind the host's back."""
+        self._check_room(tokens)
+        return self.lengths + (tokens if self.counts is None else self.counts)
 
     def append(self, key: Tensor, value: Tensor, layer_idx: int) -> None:
-        self.lengths_after(key.shape[2])  # checks the room
+        self._check_room(key.shape[2])
         tracked = {} if self.positions is None else {"positions": self.positions[layer_idx],
                                                      "next_position": self.next_position}
         paged_kv_append(self.caches[layer_idx], key, value, self.page_table, self.lengths, self.counts, **tracked)
@@ -501,12 +501,12 @@ class PagedKVState:
 
     def advance(self, tokens: int) -> None:
         """The forward's tokens are now cached in every layer."""
-        self.lengths_after(tokens)  # checks the room
+        self._check_room(tokens)
         new = tokens if self.counts is None else self.counts
         self.lengths.add_(new)
         self.next_position.add_(new)
         self.max_length += tokens
-        self.counts = self._after = None
+        self.counts = None
 
     def evict(self, keep: int, recent: int = 0) -> None:
         """`paged_kv_evict` in every layer; needs `track=True`."""
@@ -516,4 +516,4 @@ class PagedKVState:
             lengths, self.weights[i], self.positions[i] = paged_kv_evict(
                 cache, self.page_table, self.lengths, self.weights[i], keep, recent, self.positions[i], self.next_position)
         self.lengths.copy_(lengths)
-        self.max_length, self._after = min(self.max_length, keep), None
+        self.max_length = min(self.max_length, keep)

@@ -43,3 +43,27 @@ def test_absent_rows_are_hidden(dtype):
     assert got.dtype == dtype and torch.equal(got[:, 0, 0], torch.where(want == low, want, mask[0, 0, :, :6].expand(3, 6)))
     with pytest.raises(RuntimeError):
         state.hide_absent(mask[..., :4], 1, 6, dtype)
+
+
+@pytest.mark.parametrize("made,counted", [(True, True), (True, False), (False, True)])
+def test_inference_mode(made, counted):
+    """Tensors made under inference mode have no version counter; a state and its counts may be such tensors."""
+    with torch.inference_mode(made):
+        state = make_state(lengths=[5, 2])
+    with torch.inference_mode(counted):
+        counts = i32([1, 0])
+    with torch.inference_mode():
+        assert state.lengths_after(1).tolist() == [6, 3]
+        state.counts = counts
+        assert state.lengths_after(1).tolist() == [6, 2]
+        state.accumulate(torch.full((2, 4, 1, 6), 0.25), 0)
+        state.advance(1)
+        assert state.lengths.tolist() == [6, 2] == state.next_position.tolist() and state.max_length == 6
+
+
+def test_lengths_that_change_behind_the_hosts_back():
+    """What a replayed graph does to the lengths leaves no trace on the host."""
+    state = make_state(lengths=[5, 2])
+    assert state.lengths_after(1).tolist() == [6, 3]
+    state.lengths.data.add_(4)  # does not count as a new version
+    assert state.lengths_after(1).tolist() == [10, 7]

@@ -58,3 +58,84 @@ def test_dense_steps_of_a_ragged_batch_without_a_mask(name, lens, av, mask):
             assert bool((w[:, length + 1 :] == 0).all())
             assert torch.allclose(w, alone.weights[0][0], rtol=0.1, atol=2e-2)
     gemm.check_status()
+
+
+@pytest.mark.parametrize("advance", [True, False])
+def test_captured_steps_follow_the_lengths(advance):
+    """Single tokens captured after a warm-up that did not advance: every replay attends to what is cached by then, the
+    lengths moved by the graph itself or between the replays."""
+    layers = blocks("e4m3", torch.float32, True, layers=2)
+    states = [make_state("e4m3", 2, layers=2) for _ in range(2)]
+    prompt = rows(2, 20, 128, seed=2, dtype=torch.float32, spread=0.1).to(DEV)
+    steps = [rows(2, 1, 128, seed=10 + i, dtype=torch.float32, spread=0.1).to(DEV) for i in range(5)]
+    ropes = [rope([20 + i, 13 + i], 1, 2, torch.float32) for i in range(5)]
+    outs = [[], []]
+    with torch.no_grad():
+        for state in states:
+            state.counts = i32([20, 13])
+            for layer in layers:
+                layer(prompt, rope(0, 20, 2, torch.float32), causal(20, 0, 2, torch.float32), past_key_value=state)
+            state.advance(20)
+        for i in range(5):  # the eager side
+            h = steps[i]
+            for layer in layers:
+                h, _ = layer(h, ropes[i], None, past_key_value=states[0])
+            states[0].advance(1)
+            outs[0].append(h)
+        state, x, cs = states[1], steps[0].clone(), [t.clone() for t in ropes[0]]
+        saved = [[t.clone() for t in group] for group in (state.weights, state.positions)]
+
+        def forward():
+            h = x
+            for layer in layers:
+                h, _ = layer(h, cs, None, past_key_value=state)
+            return h
+
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            forward()  # warm-up
+            for group, old in zip((state.weights, state.positions), saved):
+                for t, u in zip(group, old):
+                    t.copy_(u)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                out = forward()
+                if advance:
+                    state.advance(1)
+            for i in range(5):
+                x.copy_(steps[i])
+                for t, u in zip(cs, ropes[i]):
+                    t.copy_(u)
+                g.replay()
+                if not advance:
+                    state.advance(1)
+                outs[1].append(out.clone())
+        stream.synchronize()
+    assert states[0].lengths.tolist() == [25, 18] == states[1].lengths.tolist()
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    for a, b in zip(states[0].weights + states[0].positions, states[1].weights + states[1].positions):
+        assert torch.equal(a, b)
+    gemm.check_status()
+
+
+def test_steps_under_inference_mode():
+    layer = blocks("e4m3", torch.float32, True, layers=1)[0]
+    prompt = rows(2, 20, 128, seed=2, dtype=torch.float32, spread=0.1).to(DEV)
+    step = rows(2, 1, 128, seed=3, dtype=torch.float32, spread=0.1).to(DEV)
+    got = []
+    for mode in (torch.inference_mode, torch.no_grad):
+        with mode():
+            s = make_state("e4m3", 2)
+            s.counts = i32([20, 13])
+            layer(prompt, rope(0, 20, 2, torch.float32), causal(20, 0, 2, torch.float32), past_key_value=s)
+            s.advance(20)
+            for i in range(2):
+                out, _ = layer(step, rope([20 + i, 13 + i], 1, 2, torch.float32), None, past_key_value=s)
+                s.advance(1)
+            s.evict(12, 4)
+            got.append([out, s.lengths, *s.weights, *s.positions])
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    gemm.check_status()
