@@ -412,8 +412,9 @@ class PagedKVState:
 
     counts (int32 [batch] or None): how many of the forward's tokens each sequence has (a right-padded batch); set it before
     the forward, `advance` uses it and clears it.  max_length is the host's bound on the lengths (default: their
-    maximum now): dense tensors are that long, plus the new tokens.  `lengths` and `next_position` are updated in place.  There is no backward pass: run the
-    model under torch.no_grad()."""
+    maximum now): dense tensors are that long, plus the new tokens.  `lengths`, `next_position` and the tensors of `weights`
+    and `positions` are updated in place.  There is no backward pass: run the model under torch.no_grad() or
+    torch.inference_mode()."""
 
     def __init__(self, caches: list[PagedKVCache], page_table: Tensor, lengths: Tensor | None = None,
                  max_length: int | None = None, track: bool = False):
@@ -513,7 +514,9 @@ class PagedKVState:
         if self.weights is None:
             raise RuntimeError("eviction needs the statistics of a PagedKVState with track=True")
         for i, cache in enumerate(self.caches):
-            lengths, self.weights[i], self.positions[i] = paged_kv_evict(
+            lengths, weights, positions = paged_kv_evict(
                 cache, self.page_table, self.lengths, self.weights[i], keep, recent, self.positions[i], self.next_position)
+            self.weights[i].copy_(weights)  # in place: captured steps hold on to these tensors
+            self.positions[i].copy_(positions)
         self.lengths.copy_(lengths)
         self.max_length = min(self.max_length, keep)

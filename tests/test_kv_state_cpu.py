@@ -67,3 +67,22 @@ def test_lengths_that_change_behind_the_hosts_back():
     assert state.lengths_after(1).tolist() == [6, 3]
     state.lengths.data.add_(4)  # does not count as a new version
     assert state.lengths_after(1).tolist() == [10, 7]
+
+
+def test_eviction_keeps_the_statistics_tensors(monkeypatch):
+    """A captured step writes the tensors it was captured with: eviction leaves its results there."""
+    from mase_b200 import kv_cache
+
+    def evict(cache, table, lengths, weights, keep, recent, positions, next_position):
+        return lengths.clamp(max=keep), weights.flip(-1), positions.flip(-1)
+
+    monkeypatch.setattr(kv_cache, "paged_kv_evict", evict)
+    state = make_state(lengths=[9, 2], layers=2)
+    for w in state.weights:
+        w.copy_(torch.rand_like(w))
+    held = list(state.weights) + list(state.positions)
+    want = [t.flip(-1) for t in held]
+    state.evict(5)
+    assert all(a is b for a, b in zip(held, state.weights + state.positions))
+    assert all(torch.equal(a, b) for a, b in zip(held, want))
+    assert state.lengths.tolist() == [5, 2] and state.max_length == 5

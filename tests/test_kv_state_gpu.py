@@ -139,3 +139,63 @@ def test_steps_under_inference_mode():
     for a, b in zip(*got):
         assert torch.equal(a, b)
     gemm.check_status()
+
+
+def test_captured_steps_and_eviction():
+    """A captured tracked step, replayed before and after evictions (one eager, one captured): the statistics that the
+    evictions go by are the ones that the replays add to."""
+    layer = blocks("e4m3", torch.float32, True, layers=1)[0]
+    prompt = rows(2, 20, 128, seed=2, dtype=torch.float32, spread=0.1).to(DEV)
+    steps = [rows(2, 1, 128, seed=10 + i, dtype=torch.float32, spread=0.1).to(DEV) for i in range(9)]
+    ropes = [rope([20 + i, 13 + i], 1, 2, torch.float32) for i in range(9)]
+    results = []
+    with torch.no_grad():
+        for captured in (False, True):
+            state, x, cs = make_state("e4m3", 2), steps[0].clone(), [t.clone() for t in ropes[0]]
+            state.counts = i32([20, 13])
+            layer(prompt, rope(0, 20, 2, torch.float32), causal(20, 0, 2, torch.float32), past_key_value=state)
+            state.advance(20)
+
+            def forward():
+                out, _ = layer(x, cs, None, past_key_value=state)
+                state.advance(1)
+                return out
+
+            stream = torch.cuda.Stream()
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                if captured:
+                    parts = [state.lengths, state.next_position, *state.weights, *state.positions]
+                    saved = [t.clone() for t in parts]
+                    forward(), state.evict(12, 4)  # warm-up
+                    for t, u in zip(parts, saved):
+                        t.copy_(u)
+                    c = state.caches[0]
+                    layer(prompt, rope(0, 20, 2, torch.float32), causal(20, 0, 2, torch.float32),
+                          past_key_value=(again := mb.PagedKVState([c], state.page_table)))  # the rows that moved, put back
+                    assert again.max_length == 0
+                    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+                    with torch.cuda.graph(graphs[0], stream=stream):
+                        out = forward()
+                    with torch.cuda.graph(graphs[1], stream=stream):
+                        state.evict(12, 4)
+                outs = []
+                for i in range(9):
+                    x.copy_(steps[i])
+                    for t, u in zip(cs, ropes[i]):
+                        t.copy_(u)
+                    if captured:
+                        graphs[0].replay()
+                    else:
+                        out = forward()
+                    outs.append(out.clone())
+                    if i == 3:
+                        state.evict(16, 4)
+                    if i == 6:
+                        graphs[1].replay() if captured else state.evict(12, 4)
+            stream.synchronize()
+            results.append(outs + [state.lengths, state.next_position, *state.weights, *state.positions])
+    assert state.lengths.tolist() == [14, 14]
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    gemm.check_status()
