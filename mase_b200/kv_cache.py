@@ -470,9 +470,13 @@ class PagedKVState:
                                key.dtype)
 
     def attend(self, query: Tensor, layer_idx: int, scaling: float | None = None) -> Tensor:
-        """`paged_attention` of the token that has just been appended; accumulates its weights when tracking."""
-        return paged_attention(self.caches[layer_idx], query, self.page_table, self.lengths_after(1), scaling,
-                               None if self.weights is None else self.weights[layer_idx])
+        """`paged_attention` of the token that has just been appended; accumulates its weights when tracking.  The query of
+        a sequence that has no new token (`counts` 0) is padding: it adds nothing to the statistics, and when tracking its
+        result is zeros."""
+        lengths, weights = self.lengths_after(1), None if self.weights is None else self.weights[layer_idx]
+        if weights is not None and self.counts is not None:
+            lengths = torch.where(self.counts > 0, lengths, 0)
+        return paged_attention(self.caches[layer_idx], query, self.page_table, lengths, scaling, weights)
 
     def hide_absent(self, mask: Tensor | None, tokens: int, keys: int, dtype: torch.dtype) -> Tensor:
         """An additive mask for the scores [batch, heads, tokens, keys] over the dense tensors of `update`: `mask` with the

@@ -86,3 +86,17 @@ def test_eviction_keeps_the_statistics_tensors(monkeypatch):
     assert all(a is b for a, b in zip(held, state.weights + state.positions))
     assert all(torch.equal(a, b) for a, b in zip(held, want))
     assert state.lengths.tolist() == [5, 2] and state.max_length == 5
+
+
+@pytest.mark.parametrize("track", [True, False])
+def test_a_sequence_without_a_new_token_adds_no_weight(monkeypatch, track):
+    from mase_b200 import kv_cache
+
+    seen = []
+    monkeypatch.setattr(kv_cache, "paged_attention", lambda cache, query, table, lengths, scaling, weights: seen.append((lengths, weights)))
+    state = make_state(lengths=[5, 2], track=track)
+    state.attend(None, 0)
+    state.counts = i32([0, 1])
+    state.attend(None, 0)
+    assert [n.tolist() for n, _ in seen] == [[6, 3], [0, 3] if track else [5, 3]]
+    assert all(n.dtype == torch.int32 and w is (state.weights[0] if track else None) for n, w in seen)

@@ -199,3 +199,27 @@ def test_captured_steps_and_eviction():
     for a, b in zip(*results):
         assert torch.equal(a, b)
     gemm.check_status()
+
+
+def test_tracked_step_with_an_idle_sequence():
+    """counts 0 in a step on the pages and in one on dense tensors: neither touches the idle sequence's statistics, and the
+    other's are those of the step alone."""
+    for quantized in (False, True):
+        layer = blocks("e4m3", torch.float32, True, layers=1)[0]
+        if quantized:
+            softmax_quantized(layer, False)
+        state = make_state("e4m3", 2)
+        prompt = rows(2, 20, 128, seed=2, dtype=torch.float32, spread=0.1).to(DEV)
+        step = rows(2, 1, 128, seed=3, dtype=torch.float32, spread=0.1).to(DEV)
+        with torch.no_grad():
+            state.counts = i32([20, 13])
+            layer(prompt, rope(0, 20, 2, torch.float32), causal(20, 0, 2, torch.float32), past_key_value=state)
+            state.advance(20)
+            before = state.weights[0].clone()
+            state.counts = i32([1, 0])
+            layer(step, rope([20, 13], 1, 2, torch.float32), None, past_key_value=state)
+            state.advance(1)
+        assert state.lengths.tolist() == [21, 13] == state.next_position.tolist()
+        assert torch.equal(state.weights[0][1], before[1])
+        assert torch.allclose((state.weights[0][0] - before[0]).sum(-1).cpu(), torch.full((2,), 4.0), rtol=1e-4)
+    gemm.check_status()
