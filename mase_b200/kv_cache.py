@@ -412,7 +412,9 @@ class PagedKVState:
 
     counts (int32 [batch] or None): how many of the forward's tokens each sequence has (a right-padded batch); set it before
     the forward, `advance` uses it and clears it.  max_length is the host's bound on the lengths (default: their
-    maximum now): dense tensors are that long, plus the new tokens.  `lengths`, `next_position` and the tensors of `weights`
+    maximum now): dense tensors are that long, plus the new tokens, and a mask has to be at least that wide.  `advance` adds
+    the padded number of tokens to it; `refresh()` makes it the largest length again, which the room check does by itself
+    before it refuses.  `lengths`, `next_position` and the tensors of `weights`
     and `positions` are updated in place.  There is no backward pass: run the model under torch.no_grad() or
     torch.inference_mode()."""
 
@@ -427,10 +429,10 @@ class PagedKVState:
         self.caches, self.page_table = list(caches), page_table
         if lengths is None:
             lengths, max_length = torch.zeros(page_table.shape[0], dtype=torch.int32, device=first.device), max_length or 0
-        elif max_length is None:
-            max_length = int(lengths.max()) if lengths.numel() else 0
         batch = _check_table(first, page_table, lengths)
         self.lengths, self.max_length, self.counts = lengths, max_length, None
+        if max_length is None:
+            self.refresh()
         self.capacity = page_table.shape[1] * first.page_size
         self.next_position = lengths.clone()  # positions count evicted tokens too
         self.weights = self.positions = None
@@ -446,9 +448,25 @@ class PagedKVState:
         if (c._code, c._bits) != _format_of(fmt, config):
             raise ValueError(f"layer {layer_idx}: the block's kv_cache configuration is not the format of its paged cache")
 
+    def _capturing(self) -> bool:
+        if not self.lengths.is_cuda:
+            return False
+        with _on_device(self.lengths):
+            return torch.cuda.is_current_stream_capturing()
+
+    def refresh(self) -> None:
+        """Set max_length to the largest length now.  Reads the lengths back: not while a graph is captured."""
+        self.max_length = int(self.lengths.max()) if self.lengths.numel() else 0
+
     def _check_room(self, tokens: int) -> None:
-        if self.max_length + tokens > self.capacity:
-            raise ValueError(f"{self.max_length} + {tokens} tokens do not fit a page table of {self.capacity}")
+        if self.max_length + tokens <= self.capacity:
+            return
+        if not self._capturing():  # the bound counts padded tokens too: look at the lengths before refusing
+            self.refresh()
+            after = self.lengths + (tokens if self.counts is None else self.counts)
+            if after.numel() == 0 or int(after.max()) <= self.capacity:
+                return
+        raise ValueError(f"{self.max_length} + {tokens} tokens do not fit a page table of {self.capacity}")
 
     def lengths_after(self, tokens: int) -> Tensor:
         """The lengths once the forward's tokens are cached.  Added up by every call: a sum that is kept would not be part
@@ -502,7 +520,8 @@ class PagedKVState:
         if self.counts is not None:  # rows of padding count for nothing
             live = torch.arange(t, device=p.device) < self.counts[:, None]
             p = torch.where(live[:, None, :, None], p, 0.0)
-        self.weights[layer_idx][:, :, :n] += p.view(b, heads, h // heads, t, n).sum((2, 3))
+        p = p.view(b, heads, h // heads, t, n).sum((2, 3))
+        self.weights[layer_idx][:, :, :n] += p[:, :, : self.capacity]  # padding may make the dense tensors longer than that
 
     def advance(self, tokens: int) -> None:
         """The forward's tokens are now cached in every layer."""

@@ -100,3 +100,33 @@ def test_a_sequence_without_a_new_token_adds_no_weight(monkeypatch, track):
     state.attend(None, 0)
     assert [n.tolist() for n, _ in seen] == [[6, 3], [0, 3] if track else [5, 3]]
     assert all(n.dtype == torch.int32 and w is (state.weights[0] if track else None) for n, w in seen)
+
+
+def test_room_goes_by_the_lengths_not_by_the_padding():
+    state = make_state()  # room for 64 tokens
+    for counts in ([30, 0], [0, 30]):
+        state.counts = i32(counts)
+        assert state.lengths_after(30).tolist() == [sum(x) for x in zip(state.lengths.tolist(), counts)]
+        state.advance(30)
+    assert state.lengths.tolist() == [30, 30] and state.max_length == 60
+    assert state.lengths_after(10).tolist() == [40, 40] and state.max_length == 30
+    state.advance(10)
+    state.counts = i32([24, 3])  # 30 padded tokens, of which the first sequence has 24
+    assert state.lengths_after(30).tolist() == [64, 43]
+    p = torch.full((2, 4, 30, 70), 1 / 70)  # dense tensors of 40 + 30 rows
+    state.accumulate(p, 0)
+    assert torch.allclose(state.weights[0].sum(-1), torch.tensor([[48 * 64 / 70] * 2, [6 * 43 / 70] * 2]))
+    state.advance(30)
+    assert state.lengths.tolist() == [64, 43]
+    with pytest.raises(ValueError, match="fit"):
+        state.lengths_after(1)
+    state.counts = i32([0, 1])
+    assert state.lengths_after(1).tolist() == [64, 44]
+    state.counts = None
+    state.refresh()
+    assert state.max_length == 64
+
+
+def test_a_state_of_no_sequences():
+    state = make_state(batch=0, lengths=[])
+    assert state.max_length == 0 and state.lengths_after(3).tolist() == []

@@ -223,3 +223,30 @@ def test_tracked_step_with_an_idle_sequence():
         assert torch.equal(state.weights[0][1], before[1])
         assert torch.allclose((state.weights[0][0] - before[0]).sum(-1).cpu(), torch.full((2,), 4.0), rtol=1e-4)
     gemm.check_status()
+
+
+def test_padded_chunks_fill_the_pages():
+    """Chunks whose padding reaches behind the page table, prompts one sequence after the other: as the sequence alone.
+    Projections of 60 and of 25 rows may round differently in fp32, which can move a code of one key or value by a step,
+    2**-6 of the largest element of its block, and with a weight of 1/25 or more for a value: 5e-3 of the largest output
+    leaves room for ten of those; a chunk that is cut off or misplaced changes it by its own size."""
+    layer = blocks("int8", torch.float32, True, layers=1)[0]
+    state, alone = make_state("int8", 2, width=4), make_state("int8", 1, width=4)
+    parts = [rows(2, n, 128, seed=20 + i, dtype=torch.float32, spread=0.1).to(DEV) for i, n in enumerate((30, 30, 30))]
+    with torch.no_grad():
+        for i, (counts, start) in enumerate((([0, 30], [0, 0]), ([30, 0], [0, 30]), ([34 - 4, 25], [30, 30]))):
+            state.counts = i32(counts)
+            keys = state.max_length + 30
+            mask = torch.stack([causal(30, s, 1, torch.float32)[0] if s + 30 == keys else torch.nn.functional.pad(
+                causal(30, s, 1, torch.float32)[0], (0, keys - s - 30), value=torch.finfo(torch.float32).min) for s in start])
+            out, _ = layer(parts[i], rope(start, 30, 2, torch.float32), mask, past_key_value=state)
+            state.advance(30)
+        assert state.lengths.tolist() == [60, 55] and state.max_length == 60
+        for i, n in ((0, 30), (2, 25)):
+            one, _ = layer(parts[i][1:, :n], rope(30 * (i > 0), n, 1, torch.float32), causal(n, 30 * (i > 0), 1, torch.float32),
+                           past_key_value=alone)
+            alone.advance(n)
+        assert float((out[1, :25] - one[0]).abs().max() / one.abs().max()) <= 5e-3
+        with pytest.raises(ValueError, match="fit"):
+            layer(parts[0], rope(60, 30, 2, torch.float32), None, past_key_value=state)
+    gemm.check_status()
