@@ -108,7 +108,8 @@ def _options_ptr(static_b: bool = False, a_e5m2: bool = False):
 def _status(device: torch.device) -> Tensor:
     t = _STATUS.get(device.index)
     if t is None:
-        t = _STATUS[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # check_status() clears it in place, under any mode
+            t = _STATUS[device.index] = torch.zeros(1, dtype=torch.int32, device=device)
     return t
 
 

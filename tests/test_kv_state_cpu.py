@@ -130,3 +130,17 @@ def test_room_goes_by_the_lengths_not_by_the_padding():
 def test_a_state_of_no_sequences():
     state = make_state(batch=0, lengths=[])
     assert state.max_length == 0 and state.lengths_after(3).tolist() == []
+
+
+def test_the_status_word_can_be_cleared_under_any_mode(monkeypatch):
+    """A status word made by a first call under inference mode is cleared and reported outside of it."""
+    from mase_b200 import _lib, gemm
+
+    monkeypatch.setattr(gemm, "_STATUS", {})
+    with torch.inference_mode():
+        status = gemm._status(torch.device("cpu"))
+    status.fill_(8)
+    with pytest.raises(_lib.MxqError, match="paged cache"):
+        gemm.check_status()
+    assert int(status) == 0
+    gemm.check_status()
