@@ -414,7 +414,9 @@ class PagedKVState:
     the forward, `advance` uses it and clears it.  max_length is the host's bound on the lengths (default: their
     maximum now): dense tensors are that long, plus the new tokens, and a mask has to be at least that wide.  `advance` adds
     the padded number of tokens to it; `refresh()` makes it the largest length again, which the room check does by itself
-    before it refuses.  `lengths`, `next_position` and the tensors of `weights`
+    before it refuses, and every forward on dense tensors once `advance` or `evict` has been captured into a graph.  A
+    captured forward on dense tensors has them as long as they were at its capture: a replay with longer sequences is
+    reported by `check_status()`.  `lengths`, `next_position` and the tensors of `weights`
     and `positions` are updated in place.  There is no backward pass: run the model under torch.no_grad() or
     torch.inference_mode()."""
 
@@ -431,6 +433,7 @@ class PagedKVState:
             lengths, max_length = torch.zeros(page_table.shape[0], dtype=torch.int32, device=first.device), max_length or 0
         batch = _check_table(first, page_table, lengths)
         self.lengths, self.max_length, self.counts = lengths, max_length, None
+        self._replayed = False  # a captured graph moves the lengths: max_length may be anything by the next forward
         if max_length is None:
             self.refresh()
         self.capacity = page_table.shape[1] * first.page_size
@@ -482,10 +485,14 @@ class PagedKVState:
 
     def update(self, key: Tensor, value: Tensor, layer_idx: int, cache_kwargs=None) -> tuple[Tensor, Tensor]:
         """Write new keys and values and return all cached ones as dense tensors (the call of a key/value cache)."""
+        if self._replayed and not self._capturing():
+            self.refresh()
         self.append(key, value, layer_idx)
-        tokens = key.shape[2]
-        return paged_kv_gather(self.caches[layer_idx], self.page_table, self.lengths_after(tokens), self.max_length + tokens,
-                               key.dtype)
+        cache, tokens = self.caches[layer_idx], key.shape[2]
+        keys, after = self.max_length + tokens, self.lengths_after(tokens)
+        # a length that the dense tensors do not cover (a graph replayed beyond what it was captured for) is reported
+        _status(cache.device).masked_fill_((after > keys).any(), 8)
+        return paged_kv_gather(cache, self.page_table, after, keys, key.dtype)
 
     def attend(self, query: Tensor, layer_idx: int, scaling: float | None = None) -> Tensor:
         """`paged_attention` of the token that has just been appended; accumulates its weights when tracking.  The query of
@@ -531,6 +538,7 @@ class PagedKVState:
         self.next_position.add_(new)
         self.max_length += tokens
         self.counts = None
+        self._replayed |= self._capturing()
 
     def evict(self, keep: int, recent: int = 0) -> None:
         """`paged_kv_evict` in every layer; needs `track=True`."""
@@ -543,3 +551,4 @@ class PagedKVState:
             self.positions[i].copy_(positions)
         self.lengths.copy_(lengths)
         self.max_length = min(self.max_length, keep)
+        self._replayed |= self._capturing()

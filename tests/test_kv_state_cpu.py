@@ -144,3 +144,47 @@ def test_the_status_word_can_be_cleared_under_any_mode(monkeypatch):
         gemm.check_status()
     assert int(status) == 0
     gemm.check_status()
+
+
+def test_the_bound_after_captured_steps(monkeypatch):
+    """A captured advance or eviction runs on the host once, and on the lengths with every replay: the dense length of the
+    next forward goes by the lengths."""
+    from mase_b200 import gemm, kv_cache
+
+    asked = []
+    monkeypatch.setattr(gemm, "_STATUS", {})
+    monkeypatch.setattr(kv_cache, "paged_kv_append", lambda *a, **k: None)
+    monkeypatch.setattr(kv_cache, "paged_kv_gather", lambda cache, table, after, keys, dtype: asked.append((after.tolist(), keys)))
+    monkeypatch.setattr(kv_cache, "paged_kv_evict", lambda c, t, n, w, keep, recent, p, x: (n.clamp(max=keep), w, p))
+    row = torch.zeros(2, 2, 3, 8)
+    for step in (lambda s: s.advance(1), lambda s: s.evict(4)):
+        state = make_state(lengths=[9, 5])
+        state.update(row, row, 0)
+        with monkeypatch.context() as m:
+            m.setattr(state, "_capturing", lambda: True)
+            before = state.lengths.clone()
+            step(state)
+            state.lengths.copy_(before)  # a capture executes nothing
+            state.update(row, row, 0)  # and cannot look at the lengths
+        bound = state.max_length
+        state.lengths.copy_(i32([20, 11]))  # replays
+        state.update(row, row, 0)
+        assert asked == [([12, 8], 12), ([12, 8], bound + 3), ([23, 14], 23)] and state.max_length == 20
+        asked.clear()
+        gemm._STATUS.clear()
+
+
+def test_lengths_beyond_the_dense_tensors_are_reported(monkeypatch):
+    from mase_b200 import _lib, gemm, kv_cache
+
+    monkeypatch.setattr(gemm, "_STATUS", {})
+    monkeypatch.setattr(kv_cache, "paged_kv_append", lambda *a, **k: None)
+    monkeypatch.setattr(kv_cache, "paged_kv_gather", lambda *a: None)
+    row = torch.zeros(2, 2, 3, 8)
+    state = make_state(lengths=[9, 5])
+    state.update(row, row, 0)
+    gemm.check_status()
+    state.lengths.data.add_(1)
+    state.update(row, row, 0)
+    with pytest.raises(_lib.MxqError, match="paged cache"):
+        gemm.check_status()

@@ -250,3 +250,46 @@ def test_padded_chunks_fill_the_pages():
         with pytest.raises(ValueError, match="fit"):
             layer(parts[0], rope(60, 30, 2, torch.float32), None, past_key_value=state)
     gemm.check_status()
+
+
+def test_a_chunk_after_replayed_steps():
+    """Captured single tokens, replayed, then a prompt chunk on dense tensors: as with steps that were not captured."""
+    layer = blocks("e4m3", torch.float32, True, layers=1)[0]
+    prompt = rows(2, 20, 128, seed=2, dtype=torch.float32, spread=0.1).to(DEV)
+    step = rows(2, 1, 128, seed=3, dtype=torch.float32, spread=0.1).to(DEV)
+    chunk = rows(2, 7, 128, seed=4, dtype=torch.float32, spread=0.1).to(DEV)
+    cs, outs = rope(20, 1, 2, torch.float32), []
+    with torch.no_grad():
+        for captured in (False, True):
+            state = make_state("e4m3", 2)
+            layer(prompt, rope(0, 20, 2, torch.float32), causal(20, 0, 2, torch.float32), past_key_value=state)
+            state.advance(20)
+
+            def forward():
+                layer(step, cs, None, past_key_value=state)
+                state.advance(1)
+
+            if captured:
+                stream = torch.cuda.Stream()
+                stream.wait_stream(torch.cuda.current_stream())
+                with torch.cuda.stream(stream):
+                    forward()
+                    g = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(g, stream=stream):
+                        forward()
+                    for _ in range(4):
+                        g.replay()
+                stream.synchronize()
+                state.refresh()
+            else:
+                for _ in range(5):
+                    forward()
+            assert state.max_length == 25
+            outs.append(layer(chunk, rope(25, 7, 2, torch.float32), causal(7, 25, 2, torch.float32), past_key_value=state)[0])
+            state.advance(7)
+            if captured:
+                g.replay()
+                outs.append(layer(chunk, rope(33, 7, 2, torch.float32), causal(7, 33, 2, torch.float32), past_key_value=state)[1])
+                assert outs.pop().shape[-1] == 40
+    assert torch.equal(*outs)
+    gemm.check_status()
