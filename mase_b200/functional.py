@@ -173,7 +173,8 @@ def attention_softmax(scores: Tensor, scale: float | None, mask: Tensor | None, 
     if mask is not None:
         mask = mask[:, :, :, :sk]
         if (mask.dtype != scores.dtype or mask.dim() != 4 or mask.shape[0] != b or mask.shape[1] != 1 or mask.shape[2] != sq
-                or mask.stride(3) != 1 or (b > 1 and mask.stride(0) != sq * mask.stride(2))):
+                or mask.shape[3] != sk or mask.device != scores.device or mask.stride(3) != 1 or mask.stride(2) < sk
+                or (b > 1 and mask.stride(0) != sq * mask.stride(2))):
             return None
         mask_ptr, mask_ld = mask.data_ptr(), mask.stride(2)
     x = scores.contiguous()

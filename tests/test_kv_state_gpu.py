@@ -293,3 +293,26 @@ def test_a_chunk_after_replayed_steps():
                 assert outs.pop().shape[-1] == 40
     assert torch.equal(*outs)
     gemm.check_status()
+
+
+def test_masks_that_the_fused_softmax_does_not_take():
+    """A mask with fewer columns than there are keys (a view whose memory goes on behind them), on another device, or with
+    rows that share memory is left to the separate operations, which broadcast or refuse it."""
+    from mase_b200 import functional as F
+
+    scores = torch.randn(1, 4, 3, 64, device=DEV)
+    wide = torch.randn(1, 1, 3, 96, device=DEV)
+    fused = lambda mask: F.attention_softmax(scores, 0.5, mask, None, None, None, None)  # noqa: E731
+    assert fused(wide[..., :40]) is None and fused(wide[..., :1]) is None and fused(wide[..., :64].cpu()) is None
+    assert fused(wide[:, :, :1, :64].expand(1, 1, 3, 64)) is None
+    assert torch.allclose(fused(wide), torch.softmax(scores * 0.5 + wide[..., :64], -1), atol=1e-6)
+    layer = blocks("e4m3", torch.float32, True, layers=1)[0]
+    h = rows(1, 32, 128, seed=2, dtype=torch.float32, spread=0.1).to(DEV)
+    m = torch.randn(1, 1, 1, 32, device=DEV)
+    with torch.no_grad():
+        for bad in (causal(32, 0, 1, torch.float32)[..., :20], causal(32, 0, 1, torch.float32).cpu()):
+            with pytest.raises(RuntimeError):
+                layer(h, rope(0, 32, 1, torch.float32), bad)
+        cs = rope(0, 32, 1, torch.float32)
+        a, b = (layer(h, cs, x)[0] for x in (m.expand(1, 1, 32, 32), m.expand(1, 1, 32, 32).contiguous()))
+    assert torch.allclose(a, b, atol=1e-5 * float(b.abs().max()))
