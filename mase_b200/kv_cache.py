@@ -88,7 +88,7 @@ class PagedKVCache:
 
     `fmt` / `config` are those of the attention blocks' `kv_cache` entry: "mxfp" with data_in_exponent_width /
     data_in_frac_width (4, 3), (5, 2) or (2, 1); "mxint" with data_in_width 2..8; blocks of 32.  head_dim 32, 64, 128 or
-    256, page_size 16, 32, 64, 128 or 256."""
+    256, page_size 16, 32, 64, 128 or 256.  The four tensors may be written in place but not exchanged."""
 
     def __init__(self, num_pages: int, num_kv_heads: int, head_dim: int, page_size: int = 64, fmt: str | None = None,
                  config: dict | None = None, device=None):
@@ -143,7 +143,7 @@ class PagedKVCache:
             if not t.is_contiguous() or t.data_ptr() % 16 or t.device != key.device:
                 raise ValueError("pages and scales are contiguous, 16-byte aligned and on one device")
         self.fmt, self.config = (None, None) if code == _lib.CACHE_BF16 else (fmt, dict(config))
-        self.key, self.value, self.key_scales, self.value_scales = key, value, key_scales, value_scales
+        self._tensors = key, value, key_scales, value_scales  # kept for as long as _desc points at them
         self.num_pages, self.num_kv_heads, self.page_size = key.shape[:3]
         self.head_dim, self.device, self._index = dim, key.device, key.device.index
         self._code, self._bits = code, bits
@@ -152,6 +152,12 @@ class PagedKVCache:
                                      self.num_kv_heads, dim, self.page_size, 0)
         self._addr = ctypes.addressof(self._desc)
         _status(self.device)  # made here, not during a capture
+
+    # The pages cannot be exchanged: the calls go by the addresses taken above.  `from_pages` makes a cache of other tensors.
+    key = property(lambda self: self._tensors[0])
+    value = property(lambda self: self._tensors[1])
+    key_scales = property(lambda self: self._tensors[2])
+    value_scales = property(lambda self: self._tensors[3])
 
     def _log2_tab(self, dtype: torch.dtype):
         if self._code == _lib.CACHE_BF16:

@@ -188,3 +188,15 @@ def test_lengths_beyond_the_dense_tensors_are_reported(monkeypatch):
     state.update(row, row, 0)
     with pytest.raises(_lib.MxqError, match="paged cache"):
         gemm.check_status()
+
+
+def test_the_pages_of_a_cache_cannot_be_exchanged():
+    """The calls go by the tensors' addresses, so a cache keeps the tensors it was made with."""
+    cache = mb.PagedKVCache.__new__(mb.PagedKVCache)
+    cache._tensors = tuple(torch.zeros(1) for _ in range(4))
+    for i, name in enumerate(("key", "value", "key_scales", "value_scales")):
+        assert getattr(cache, name) is cache._tensors[i]
+        with pytest.raises(AttributeError):
+            setattr(cache, name, torch.zeros(1))
+        with pytest.raises(AttributeError):
+            delattr(cache, name)
