@@ -124,6 +124,11 @@ at::Tensor mx_fake(const at::Tensor &x, int64_t kind, int64_t block, int64_t p0,
 bool on(const at::Tensor &t, int64_t device) { return t.is_cuda() && t.device().index() == device; }
 bool float_type(const at::Tensor &t) { return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16; }
 
+// a gradient or a tangent that the calls would drop
+bool differentiated(const at::Tensor &t) {
+  return (t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined();
+}
+
 bool plain_table(const at::Tensor &table, const at::Tensor &lengths, int64_t device) {
   return on(table, device) && on(lengths, device) && table.scalar_type() == at::kInt && lengths.scalar_type() == at::kInt &&
          table.dim() == 2 && lengths.dim() == 1 && table.size(0) == lengths.size(0) && table.size(0) > 0 &&
@@ -136,7 +141,7 @@ bool plain_vector(const c10::optional<at::Tensor> &t, int64_t n, int64_t device)
 }
 bool plain_stats(const at::Tensor &t, at::ScalarType type, int64_t batch, int64_t heads, int64_t device) {
   return on(t, device) && t.scalar_type() == type && t.dim() == 3 && t.size(0) == batch && t.size(1) == heads &&
-         t.size(2) > 0 && t.is_contiguous();
+         t.size(2) > 0 && t.is_contiguous() && !differentiated(t);
 }
 void *ptr(const c10::optional<at::Tensor> &t) { return t.has_value() ? t->data_ptr() : nullptr; }
 
@@ -145,7 +150,7 @@ c10::optional<at::Tensor> paged_attention(int64_t cache, int64_t device, const a
                                           const at::Tensor &status) {
   const auto *c = reinterpret_cast<const mxq_paged_cache *>(cache);
   const int64_t nd = query.dim();
-  if (!on(query, device) || !float_type(query) || (query.requires_grad() && at::GradMode::is_enabled()) ||
+  if (!on(query, device) || !float_type(query) || differentiated(query) ||
       !plain_table(table, lengths, device) || (nd != 3 && nd != 4) || (nd == 4 && query.size(2) != 1) ||
       query.size(0) != table.size(0) || query.size(nd - 1) != c->head_dim || query.stride(nd - 1) != 1 ||
       query.size(1) < 1 || query.size(1) % c->heads != 0)
@@ -183,7 +188,7 @@ bool paged_append(int64_t cache, int64_t device, const at::Tensor &key, const at
                   const at::Tensor &status) {
   const auto *c = reinterpret_cast<const mxq_paged_cache *>(cache);
   if (!on(key, device) || !on(value, device) || !float_type(key) || value.scalar_type() != key.scalar_type() ||
-      (at::GradMode::is_enabled() && (key.requires_grad() || value.requires_grad())) ||
+      differentiated(key) || differentiated(value) ||
       !plain_table(table, lengths, device) || key.dim() != 4 || key.sizes() != value.sizes() ||
       key.size(0) != table.size(0) || key.size(1) != c->heads || key.size(3) != c->head_dim || key.numel() == 0 ||
       !plain_rows(key) || !plain_rows(value))

@@ -27,6 +27,7 @@ import ctypes
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from . import gemm
@@ -167,6 +168,13 @@ class PagedKVCache:
         return _ceil_tab_ptr(dtype) if self._code == _lib.CACHE_INT8 else _floor_tab_ptr()
 
 
+def _no_autograd(what: str, *tensors: Tensor | None) -> None:
+    """Raises when one of the tensors carries a gradient or, in forward mode, a tangent: the calls would drop it."""
+    for t in tensors:
+        if t is not None and ((t.requires_grad and torch.is_grad_enabled()) or forward_ad.unpack_dual(t).tangent is not None):
+            raise NotImplementedError(f"{what} has no derivative: call it under torch.no_grad() on tensors without a tangent")
+
+
 def _check_table(cache: PagedKVCache, page_table: Tensor, lengths: Tensor) -> int:
     """Checks a page table [batch, width] and the lengths [batch]; returns the batch size."""
     if page_table.dtype != torch.int32 or lengths.dtype != torch.int32:
@@ -231,8 +239,7 @@ def paged_kv_append(cache: PagedKVCache, key: Tensor, value: Tensor, page_table:
     if key.dtype not in _DT or value.dtype != key.dtype:
         raise NotImplementedError(f"paged_kv_append: dtypes {key.dtype} / {value.dtype} are not supported "
                                   "(float32 and bfloat16 are, the same for both)")
-    if torch.is_grad_enabled() and (key.requires_grad or value.requires_grad):
-        raise NotImplementedError("a paged cache has no backward pass: append to it under torch.no_grad()")
+    _no_autograd("paged_kv_append", key, value)
     batch = _check_table(cache, page_table, lengths)
     if key.dim() != 4 or key.shape != value.shape or key.shape[0] != batch or key.shape[1] != cache.num_kv_heads \
             or key.shape[3] != cache.head_dim:
@@ -311,8 +318,7 @@ def paged_attention(cache: PagedKVCache, query: Tensor, page_table: Tensor, leng
     _require_cuda(query, "paged_attention")
     if query.dtype not in _DT:
         raise NotImplementedError(f"paged_attention: dtype {query.dtype} is not supported (float32 and bfloat16 are)")
-    if query.requires_grad and torch.is_grad_enabled():
-        raise NotImplementedError("paged_attention has no backward pass: call it under torch.no_grad()")
+    _no_autograd("paged_attention", query, weights)
     batch = _check_table(cache, page_table, lengths)
     if query.dim() == 4:
         if query.shape[2] != 1:
@@ -372,6 +378,7 @@ def paged_kv_evict(cache: PagedKVCache, page_table: Tensor, lengths: Tensor, wei
         _check_every_call(cache)
         return got
     _require_cuda(weights, "paged_kv_evict")
+    _no_autograd("paged_kv_evict", weights)
     batch = _check_table(cache, page_table, lengths)
     _check_stats(weights, "weights", torch.float32, batch, cache)
     width = weights.shape[2]

@@ -200,3 +200,21 @@ def test_the_pages_of_a_cache_cannot_be_exchanged():
             setattr(cache, name, torch.zeros(1))
         with pytest.raises(AttributeError):
             delattr(cache, name)
+
+
+def test_derivatives_are_refused():
+    from torch.autograd import forward_ad
+
+    from mase_b200.kv_cache import _no_autograd
+
+    x = torch.zeros(3)
+    _no_autograd("call", x, None)
+    with pytest.raises(NotImplementedError, match="call has no derivative"):
+        _no_autograd("call", x, torch.zeros(3, requires_grad=True))
+    with torch.no_grad():
+        _no_autograd("call", torch.zeros(3, requires_grad=True))
+    with forward_ad.dual_level():
+        _no_autograd("call", x)
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode(), pytest.raises(NotImplementedError, match="call has no derivative"):
+                _no_autograd("call", forward_ad.make_dual(x, x))

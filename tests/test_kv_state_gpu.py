@@ -316,3 +316,25 @@ def test_masks_that_the_fused_softmax_does_not_take():
         cs = rope(0, 32, 1, torch.float32)
         a, b = (layer(h, cs, x)[0] for x in (m.expand(1, 1, 32, 32), m.expand(1, 1, 32, 32).contiguous()))
     assert torch.allclose(a, b, atol=1e-5 * float(b.abs().max()))
+
+
+def test_derivatives_are_refused_by_the_calls():
+    from torch.autograd import forward_ad
+
+    state = make_state("e4m3", 2)
+    cache, table, lens = state.caches[0], state.page_table, i32([3, 4])
+    q, kv, w = torch.zeros(2, 4, 1, 32, device=DEV), torch.zeros(2, 2, 1, 32, device=DEV), torch.zeros(2, 2, 16, device=DEV)
+    calls = [lambda f: mb.paged_attention(cache, f(q), table, lens), lambda f: mb.paged_attention(cache, q, table, lens, weights=f(w)),
+             lambda f: mb.paged_kv_append(cache, f(kv), kv, table, lens), lambda f: mb.paged_kv_append(cache, kv, f(kv), table, lens),
+             lambda f: mb.paged_kv_evict(cache, table, lens, f(w), 2)]
+    with forward_ad.dual_level():
+        for call in calls:
+            call(lambda t: t)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="no derivative"):
+                call(lambda t: forward_ad.make_dual(t, torch.ones_like(t)))
+    for call in calls:
+        with pytest.raises(NotImplementedError, match="no derivative"):
+            call(lambda t: t.clone().requires_grad_())
+        with torch.no_grad():
+            call(lambda t: t.clone().requires_grad_())
+    gemm.check_status()
