@@ -169,19 +169,18 @@ class _AttentionMX(nn.Module):
         # only the quantized operand is known to fit tf32; the other one takes the fp32 split
         weights = self._product(query, key, exact=False)
         dropout = self.training and self.attention_dropout > 0
+        tracked = paged is not None and paged.weights is not None  # goes by the softmax before dropout and its quantizer
         if paged is not None:  # the dense tensors are as long as the longest sequence may be
             attention_mask = paged.hide_absent(attention_mask, input_shape[-1], key.shape[-2], weights.dtype)
         # scaling, mask, the softmax with its input quantizer and the quantizer of the probabilities: one kernel
+        apart = dropout or tracked  # the quantizer of the probabilities by itself
         fused = F_mx.attention_softmax(weights, self.scaling, attention_mask,
                                        None if self.softmax_bypass else "minifloat", self.softmax_config,
-                                       None if self.av_bypass or dropout else self._format, self.av_config)
+                                       None if self.av_bypass or apart else self._format, self.av_config)
         if fused is not None:
             weights = fused
-            if dropout:
-                weights = nn.functional.dropout(weights, p=self.attention_dropout, training=True)
-                if not self.av_bypass:
-                    weights = self._quantize(weights, self.av_config)
         else:
+            apart = True
             weights = weights * self.scaling
             if attention_mask is not None:
                 weights = weights + attention_mask[:, :, :, : key.shape[-2]]
@@ -189,12 +188,12 @@ class _AttentionMX(nn.Module):
                 weights = F_mx.softmax_minifloat(weights, self.softmax_config, dim=-1)
             else:
                 weights = torch.softmax(weights.to(torch.float32), dim=-1).to(weights.dtype)
-            if dropout:
-                weights = nn.functional.dropout(weights, p=self.attention_dropout, training=True)
-            if not self.av_bypass:
-                weights = self._quantize(weights, self.av_config)
-        if paged is not None:
+        if tracked:
             paged.accumulate(weights, self.layer_idx)
+        if dropout:
+            weights = nn.functional.dropout(weights, p=self.attention_dropout, training=True)
+        if apart and not self.av_bypass:
+            weights = self._quantize(weights, self.av_config)
         out = self._product(weights, value.transpose(2, 3).contiguous(), exact=False)  # [B, H, S, D]
         out = out.transpose(1, 2).contiguous().reshape(*input_shape, -1)
         return self.o_proj(out), weights

@@ -529,8 +529,8 @@ class PagedKVState:
         return torch.where(absent, torch.finfo(mask.dtype).min, mask[:, :, :, :keys])
 
     def accumulate(self, probabilities: Tensor, layer_idx: int) -> None:
-        """Add dense softmax weights [batch, heads, tokens, keys] of the forward's tokens to the statistics of the tokens
-        that each sequence has."""
+        """Add dense softmax weights [batch, heads, tokens, keys] of the forward's tokens (before dropout and the quantizer
+        of the probabilities, as `attend` counts them) to the statistics of the tokens that each sequence has."""
         if self.weights is None:
             return
         b, h, t, n = probabilities.shape

@@ -338,3 +338,29 @@ def test_derivatives_are_refused_by_the_calls():
         with torch.no_grad():
             call(lambda t: t.clone().requires_grad_())
     gemm.check_status()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dropout", [0.0, 0.5])
+def test_statistics_are_those_of_the_plain_softmax(dropout, dtype):
+    """Dense forwards count the softmax weights, one unit a query, not what the quantizer of the probabilities (here four
+    bits) or dropout makes of them; and tracking changes no output.  The softmax is fp32; a bf16 weight is off by at most
+    2**-9 of itself on one side, so is their sum."""
+    layer = softmax_quantized(blocks("e4m3", dtype, True, layers=1)[0], True)
+    layer.av_config = CONFIGS["e2m1"][1]
+    layer.attention_dropout = dropout
+    layer.train(dropout > 0)
+    h = rows(2, 64, 128, seed=2, dtype=dtype, spread=0.1).to(DEV)
+    outs = []
+    for track in (True, False):
+        state = make_state("e4m3", 2, track=track)
+        with torch.no_grad():
+            torch.manual_seed(5)
+            outs.append(layer(h, rope(0, 64, 2, dtype), causal(64, 0, 2, dtype), past_key_value=state))
+        if track:
+            got = state.weights[0][:, :, :64].sum(-1)
+            rel = 1e-5 if dtype == torch.float32 else 2.0 ** -9
+            assert bool(((got / 256 - 1).abs() <= rel + 1e-5).all()), got
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    assert not torch.allclose(outs[0][1].float().sum(-1), torch.ones((), device=DEV), rtol=1e-2)  # the quantizer shows
+    gemm.check_status()
