@@ -3,6 +3,7 @@
 // output and the activation scratch from torch's allocator, takes torch's current stream and calls libmxq; nothing
 // here computes.  mase_b200.gemm uses it when it is built and otherwise issues the same C calls through ctypes.
 
+#include <algorithm>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -155,8 +156,12 @@ c10::optional<at::Tensor> paged_attention(int64_t cache, int64_t device, const a
       query.size(0) != table.size(0) || query.size(nd - 1) != c->head_dim || query.stride(nd - 1) != 1 ||
       query.size(1) < 1 || query.size(1) % c->heads != 0)
     return c10::nullopt;
-  const int64_t batch = query.size(0), heads = query.size(1), width = table.size(1);
-  if (weights.has_value() && !plain_stats(*weights, at::kFloat, batch, c->heads, device)) return c10::nullopt;
+  const int64_t batch = query.size(0), heads = query.size(1);
+  int64_t width = table.size(1);
+  if (weights.has_value()) {
+    if (!plain_stats(*weights, at::kFloat, batch, c->heads, device)) return c10::nullopt;
+    width = std::min(width, (weights->size(2) + c->page_size - 1) / c->page_size);  // no scores behind the statistics
+  }
   const c10::cuda::CUDAGuard guard(query.device());
   const int64_t n_ws = mxq_paged_attention_workspace_bytes(c, batch, heads, width, weights.has_value());
   if (n_ws < 0) return c10::nullopt;

@@ -307,7 +307,9 @@ def paged_attention(cache: PagedKVCache, query: Tensor, page_table: Tensor, leng
     query's shape and dtype; a sequence of length 0 gives zeros.  Softmax and sums in fp32.
 
     `weights` (fp32 [batch, num_kv_heads, width], width at least the largest length) accumulates in place: the softmax
-    weight of every cached token, summed over the query heads of its key/value head, is added to its entry."""
+    weight of every cached token, summed over the query heads of its key/value head, is added to its entry.  The call then
+    takes a workspace of 4 bytes a query head (a group's rounded up to a power of two) and slot of the narrower of page
+    table and `weights`, whatever the lengths are: give neither more columns than the sequences may need."""
     if scaling is None:
         scaling = cache.head_dim ** -0.5
     ext = _binding()
@@ -340,6 +342,8 @@ def paged_attention(cache: PagedKVCache, query: Tensor, page_table: Tensor, leng
         q = q.contiguous()
     lib = _lib.lib()
     heads, width = q.shape[1], page_table.shape[1]
+    if weights is not None:  # the workspace holds scores for every slot of the table: none behind the statistics
+        width = min(width, -(-weights.shape[2] // cache.page_size))
     n_ws = int(lib.mxq_paged_attention_workspace_bytes(cache._addr, batch, heads, width, 0 if weights is None else 1))
     if n_ws < 0:
         _lib.check(n_ws, "mxq_paged_attention_workspace_bytes")

@@ -364,3 +364,33 @@ def test_statistics_are_those_of_the_plain_softmax(dropout, dtype):
     assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
     assert not torch.allclose(outs[0][1].float().sum(-1), torch.ones((), device=DEV), rtol=1e-2)  # the quantizer shows
     gemm.check_status()
+
+
+@pytest.mark.parametrize("binding", [True, False])
+def test_the_workspace_of_a_tracked_step_follows_the_statistics(monkeypatch, binding):
+    """A page table far wider than the statistics: the same results and a workspace for the statistics' slots only; lengths
+    behind them are reported as before."""
+    from mase_b200 import _lib, kv_cache
+
+    if not binding:
+        monkeypatch.setattr(kv_cache, "_BINDING", False)
+    fmt, cfg = CONFIGS["e4m3"]
+    cache = mb.PagedKVCache(13, 2, 64, 16, fmt, cfg, DEV)
+    table = torch.full((3, 40000), -1, dtype=torch.int32)
+    table[:, :4] = torch.arange(12).view(3, 4)
+    table = table.to(DEV)
+    k = rows(3, 2, 50, 64, seed=1, dtype=torch.bfloat16).to(DEV)
+    mb.paged_kv_append(cache, k, k, table, i32([0, 0, 0]))
+    q, lens = rows(3, 8, 64, seed=2, dtype=torch.bfloat16).to(DEV), i32([50, 0, 33])
+    want_w = torch.zeros(3, 2, 50, device=DEV)
+    want = mb.paged_attention(cache, q, table[:, :4].contiguous(), lens, weights=want_w)
+    w = torch.zeros(3, 2, 50, device=DEV)
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = mb.paged_attention(cache, q, table, lens, weights=w)
+    assert torch.cuda.max_memory_allocated() - before < 8 << 20  # 3 x 40000 x 16 slots of 8 heads of scores: 61 MB
+    assert torch.equal(got, want) and torch.equal(w, want_w)
+    gemm.check_status()
+    mb.paged_attention(cache, q, table, i32([51, 0, 33]), weights=w)
+    with pytest.raises(_lib.MxqError, match="paged cache"):
+        gemm.check_status()
