@@ -181,7 +181,7 @@ def _check_table(cache: PagedKVCache, page_table: Tensor, lengths: Tensor) -> in
         raise NotImplementedError("page_table and lengths are int32")
     if page_table.dim() != 2 or lengths.dim() != 1 or page_table.shape[0] != lengths.shape[0]:
         raise ValueError("page_table is [batch, width] and lengths [batch]")
-    if page_table.shape[1] < 1 or page_table.stride(1) != 1:
+    if page_table.shape[1] < 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
         raise ValueError("page_table has at least one column and contiguous rows")
     if page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]:
         raise ValueError("the rows of page_table may not overlap")

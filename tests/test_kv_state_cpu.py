@@ -218,3 +218,14 @@ def test_derivatives_are_refused():
         for mode in (torch.enable_grad, torch.no_grad):
             with mode(), pytest.raises(NotImplementedError, match="call has no derivative"):
                 _no_autograd("call", forward_ad.make_dual(x, x))
+
+
+def test_page_tables_of_one_column_have_no_column_stride():
+    from mase_b200.kv_cache import _check_table
+
+    cache = SimpleNamespace(device=torch.device("cpu"))
+    wide = torch.zeros(3, 8, dtype=torch.int32)
+    assert _check_table(cache, wide[:, ::8], i32([1, 2, 3])) == 3 and wide[:, ::8].stride(1) == 8
+    assert _check_table(cache, wide[:1, ::8].t(), i32([1])) == 1
+    with pytest.raises(ValueError, match="contiguous rows"):
+        _check_table(cache, wide[:, ::2], i32([1, 2, 3]))

@@ -394,3 +394,18 @@ def test_the_workspace_of_a_tracked_step_follows_the_statistics(monkeypatch, bin
     mb.paged_attention(cache, q, table, i32([51, 0, 33]), weights=w)
     with pytest.raises(_lib.MxqError, match="paged cache"):
         gemm.check_status()
+
+
+def test_page_table_of_one_strided_column():
+    fmt, cfg = CONFIGS["int8"]
+    cache = mb.PagedKVCache(3, 2, 64, 16, fmt, cfg, DEV)
+    table = torch.full((3, 8), -1, dtype=torch.int32, device=DEV)
+    table[:, 0] = i32([2, 0, 1])
+    k, lens = rows(3, 2, 9, 64, seed=1, dtype=torch.bfloat16).to(DEV), i32([9, 0, 4])
+    q, got = rows(3, 8, 64, seed=2, dtype=torch.bfloat16).to(DEV), []
+    for t in (table[:, ::8], table[:, :1].contiguous()):
+        mb.paged_kv_append(cache, k, k, t, i32([0, 0, 0]))
+        got.append([mb.paged_attention(cache, q, t, lens), *mb.paged_kv_gather(cache, t, lens, 9)])
+    gemm.check_status()
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
