@@ -230,10 +230,11 @@ struct Worker {
     }
   }
 
-  // x - m in units of log2; fp32 queries take the factor scaling * log2(e) with 48 bits
+  // x - m in units of log2; fp32 queries take the factor scaling * log2(e) with 48 bits (an infinite score only the first term:
+  // the second one may be zero or of the other sign)
   static __device__ __forceinline__ float score(float s, float c_hi, float c_lo, float m) {
     const float x = fmaf(s, c_hi, -m);
-    return Elem<T>::kBf16 ? x : fmaf(s, c_lo, x);
+    return Elem<T>::kBf16 || fabsf(x) == INFINITY ? x : fmaf(s, c_lo, x);
   }
 
   // One tile from a stage of the ring; `live` tokens of it exist.
@@ -280,7 +281,11 @@ struct Worker {
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[n][i] += kTerms > 1 ? s_odd[n][i] + s_low[n][i] : s_odd[n][i];
+      for (int i = 0; i < 4; ++i) {
+        const float high = s[n][i] + s_odd[n][i];  // of the first terms
+        // an infinite key has this score; the lower terms, zero or of the other sign, would make it NaN
+        s[n][i] = kTerms == 1 || fabsf(high) == INFINITY ? high : s[n][i] + (s_odd[n][i] + s_low[n][i]);
+      }
     // rows: tokens r (entries 0, 1) and r + 8 (2, 3); columns: heads 2t, 2t + 1
     float x[NT][4], top = kLowest;
 #pragma unroll

@@ -304,7 +304,8 @@ def paged_attention(cache: PagedKVCache, query: Tensor, page_table: Tensor, leng
     query [batch, heads, 1, head_dim] (or [batch, heads, head_dim]), fp32 or bf16; heads is a multiple of the cache's
     num_kv_heads, query heads h * group .. h * group + group - 1 read key/value head h (what `repeat_kv` lays out).
     `lengths` counts the new token when it has been appended.  scaling: default head_dim ** -0.5.  The result has the
-    query's shape and dtype; a sequence of length 0 gives zeros.  Softmax and sums in fp32.
+    query's shape and dtype; a sequence of length 0 gives zeros.  Softmax and sums in fp32.  Queries and values are finite
+    (an infinite value makes its element of the result NaN); a key whose score is -inf has weight 0.
 
     `weights` (fp32 [batch, num_kv_heads, width], width at least the largest length) accumulates in place: the softmax
     weight of every cached token, summed over the query heads of its key/value head, is added to its entry.  The call then
