@@ -226,7 +226,8 @@ def paged_kv_append(cache: PagedKVCache, key: Tensor, value: Tensor, page_table:
     sequence b goes to slot lengths[b] + t.  `counts` (int32 [batch]): only the first counts[b] tokens of sequence b exist
     (a padded batch).  Codes and shared exponents are those of `mxfp_quantizer` / `mxint_quantizer` along head_dim.
     `lengths` is not changed: add the new tokens to it once every layer has them.  The pages that are written belong to one
-    sequence of the batch each.
+    sequence of the batch each.  Rows are finite: no code stands for an infinity or NaN, and what a block of 32 with one in
+    it holds means nothing (other blocks are not touched by it).
 
     `positions` (int32 [batch, num_kv_heads, width]) is the record of token positions that `paged_kv_evict` keeps: the
     entries of the new slots become next_position[b] + t (int32 [batch]; default: lengths[b] + t)."""
@@ -272,8 +273,8 @@ def paged_kv_append(cache: PagedKVCache, key: Tensor, value: Tensor, page_table:
 def paged_kv_gather(cache: PagedKVCache, page_table: Tensor, lengths: Tensor, max_length: int,
                     dtype: torch.dtype = torch.bfloat16) -> tuple[Tensor, Tensor]:
     """The cached rows as dense tensors (key, value), each [batch, num_kv_heads, max_length, head_dim] of `dtype`: what
-    `kv_cache_mxfp` / `kv_cache_mxint` made of the rows that went in.  Rows from lengths[b] on are zeros; tokens from
-    max_length on are left out."""
+    `kv_cache_mxfp` / `kv_cache_mxint` made of the rows that went in, except that MXINT mantissas hold no negative zero.
+    Rows from lengths[b] on are zeros; tokens from max_length on are left out."""
     ext = _binding()
     if ext and (got := ext.paged_gather(cache._addr, cache._index, page_table, lengths, max_length, dtype,
                                         _status(cache.device))) is not None:
