@@ -457,6 +457,8 @@ class PagedKVState:
             self.refresh()
         self.capacity = page_table.shape[1] * first.page_size
         self.next_position = lengths.clone()  # positions count evicted tokens too
+        self._slots = torch.arange(self.capacity, dtype=torch.int32, device=first.device)
+        self._slots[:1] = -1  # the first row is hidden from nobody: a softmax needs one
         self.weights = self.positions = None
         if track:
             shape = (batch, first.num_kv_heads, self.capacity)
@@ -519,20 +521,27 @@ class PagedKVState:
         result is zeros."""
         lengths, weights = self.lengths_after(1), None if self.weights is None else self.weights[layer_idx]
         if weights is not None and self.counts is not None:
-            lengths = torch.where(self.counts > 0, lengths, 0)
+            lengths = lengths.masked_fill(self.counts <= 0, 0)
         return paged_attention(self.caches[layer_idx], query, self.page_table, lengths, scaling, weights)
+
+    def _absent(self, tokens: int, keys: int) -> Tensor:
+        """[batch, 1, 1, keys]: the dense row is behind the sequence's tokens, and not its first one."""
+        slots = self._slots[:keys]
+        if keys > self.capacity:  # padded tokens
+            slots = torch.cat([slots, torch.arange(self.capacity, keys, dtype=torch.int32, device=slots.device)])
+        return slots >= self.lengths_after(tokens)[:, None, None, None]
 
     def hide_absent(self, mask: Tensor | None, tokens: int, keys: int, dtype: torch.dtype) -> Tensor:
         """An additive mask for the scores [batch, heads, tokens, keys] over the dense tensors of `update`: `mask` with the
         lowest value of its type at the rows that are behind a sequence's tokens (zeros in the dense tensors, which would
         take their share of the softmax).  A sequence without tokens keeps its first row, and gets its zeros as a result."""
-        live = self.lengths_after(tokens).clamp(min=1)[:, None, None, None]
-        absent = torch.arange(keys, device=live.device) >= live  # [batch, 1, 1, keys]
+        absent = self._absent(tokens, keys)  # [batch, 1, 1, keys]
         if mask is None:
-            mask = torch.zeros((1, 1, tokens, keys), dtype=dtype, device=live.device)
-        elif not mask.is_floating_point():
+            mask = absent.to(dtype).mul(torch.finfo(dtype).min)
+            return mask if tokens == 1 else mask.expand(-1, -1, tokens, -1).contiguous()
+        if not mask.is_floating_point():
             mask = mask.to(dtype)
-        return torch.where(absent, torch.finfo(mask.dtype).min, mask[:, :, :, :keys])
+        return mask[:, :, :, :keys].masked_fill(absent, torch.finfo(mask.dtype).min)
 
     def accumulate(self, probabilities: Tensor, layer_idx: int) -> None:
         """Add dense softmax weights [batch, heads, tokens, keys] of the forward's tokens (before dropout and the quantizer
@@ -541,11 +550,10 @@ class PagedKVState:
             return
         b, h, t, n = probabilities.shape
         heads = self.caches[layer_idx].num_kv_heads
-        there = torch.arange(n, device=probabilities.device) < self.lengths_after(t)[:, None]
-        p = torch.where(there[:, None, None, :], probabilities.detach().float(), 0.0)
+        p = probabilities.detach().float().masked_fill(self._absent(t, n), 0.0)
         if self.counts is not None:  # rows of padding count for nothing
-            live = torch.arange(t, device=p.device) < self.counts[:, None]
-            p = torch.where(live[:, None, :, None], p, 0.0)
+            padding = torch.arange(t, device=p.device) >= self.counts[:, None]
+            p = p.masked_fill(padding[:, None, :, None], 0.0)
         p = p.view(b, heads, h // heads, t, n).sum((2, 3))
         self.weights[layer_idx][:, :, :n] += p[:, :, : self.capacity]  # padding may make the dense tensors longer than that
 

@@ -409,3 +409,67 @@ def test_page_table_of_one_strided_column():
     gemm.check_status()
     for a, b in zip(*got):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_captured_dense_steps(dtype):
+    """Steps that need the dense tensors, captured with a bound that leaves room for the replays: as eager steps on tensors
+    of the same length.  A replay beyond them is reported."""
+    from mase_b200 import _lib
+
+    layer = softmax_quantized(blocks("e4m3", dtype, True, layers=1)[0], False)
+    prompt = rows(3, 20, 128, seed=2, dtype=dtype, spread=0.1).to(DEV)
+    steps = [rows(3, 1, 128, seed=10 + i, dtype=dtype, spread=0.1).to(DEV) for i in range(4)]
+    ropes = [rope([20 + i, 13 + i, 4], 1, 3, dtype) for i in range(4)]
+    results = []
+    with torch.no_grad():
+        for captured in (False, True):
+            state = make_state("e4m3", 3)
+            state.counts = i32([20, 13, 4])
+            layer(prompt, rope(0, 20, 3, dtype), causal(20, 0, 3, dtype), past_key_value=state)
+            state.advance(20)
+            x, cs, counts = steps[0].clone(), [t.clone() for t in ropes[0]], i32([1, 1, 0])
+
+            def forward():
+                state.counts = counts
+                out, p = layer(x, cs, None, past_key_value=state)
+                state.advance(1)
+                return out, p
+
+            stream = torch.cuda.Stream()
+            stream.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(stream):
+                parts = [state.lengths, state.next_position, *state.weights, *state.positions]
+                saved = [t.clone() for t in parts]
+                state.max_length = 23
+                forward()  # warm-up
+                for t, u in zip(parts, saved):
+                    t.copy_(u)
+                state.max_length = 23
+                if captured:
+                    g = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(g, stream=stream):
+                        out, p = forward()
+                outs = []
+                for i in range(4):
+                    x.copy_(steps[i])
+                    for t, u in zip(cs, ropes[i]):
+                        t.copy_(u)
+                    if captured:
+                        g.replay()
+                    else:
+                        state.max_length = 23
+                        out, p = forward()
+                    assert p.shape[-1] == 24
+                    outs += [out.clone(), p.clone()]
+            stream.synchronize()
+            gemm.check_status()
+            assert state.lengths.tolist() == [24, 17, 4]
+            results.append(outs + [*state.weights, *state.positions])
+        for a, b in zip(*results):
+            assert torch.equal(a, b)
+        with torch.cuda.stream(stream):
+            g.replay()
+        stream.synchronize()
+        with pytest.raises(_lib.MxqError, match="paged cache"):
+            gemm.check_status()
