@@ -23,7 +23,7 @@ constexpr int kThreads = 256;
 // Two neighbouring lanes share a block of 32 elements, 16 each; the codes and the shared exponent are those of the plain
 // quantizers (the bf16 routines are the ones behind mxq_mxfp_extract / mxq_mxint_extract).  Bound by the logic unit
 // (about 18 instructions an element) with reads and page lookups in flight under it: 4 x 2048 tokens x 8 heads of 128, bf16
-// to E4M3, together with the read-back of what is cached then: 28 us for 105 MB.
+// to E4M3: 19 us, and 12 us for the read-back of what is cached then (105 MB in both, 28 us in a row).
 struct AppendArgs {
   const void *src[2];
   int64_t stride_b[2], stride_h[2], stride_t[2];
@@ -88,7 +88,7 @@ struct Half<__nv_bfloat16> {
       return mxint_codes_bf16(lo, hi, tab, bits, scale);
     } else if constexpr (Format<kFormat>::kBits == 4) {
       // with the four exponents of E2M1 nearly every block has subnormal codes, which the other routine patches one by one:
-      // 16 heads x 4096 tokens of 128 with the read-back 53 us, 56 with it
+      // 16 heads x 4096 tokens of 128 with the read-back 55 us, 58 with it (E4M3 27)
       float v[16];
       uint32_t b[8], code[16];
       unpack(lo, b);
@@ -321,7 +321,7 @@ gather_kernel(const Cache c, const Table table, const int32_t *lengths, T *key, 
 // histogram in each CTA's shared memory, added up over the cluster) find the key of the last token kept, and every warp
 // then walks a contiguous part of the slots, four neighbours a lane, so that ranks follow the slot order.  Keys live in
 // shared memory when they fit and are read again from L2 otherwise.  Bound by the chain of barriers and scans, not by its
-// 16 bytes a slot: 64 rows of 16384 slots take 20 us, 8 rows of 1500 slots 6 to 9; with the moves behind it 69 and 11 us.
+// 16 bytes a slot: 64 rows of 12000 to 16384 slots take 20 us, 8 rows of 1500 slots 8; with the moves behind it 68 and 12 us.
 constexpr int kSelectThreads = 512;
 constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kBins = 2048;
@@ -577,9 +577,11 @@ evict_select_kernel(const Cache c, int64_t table_tokens, const EvictArgs a) {
 }
 
 // A warp takes `per_warp` moves at a time (up to 32): each lane looks one of them up (slots, pages) and moves its
-// statistics, then the warp copies the key and value rows of all of them, 16 bytes a lane with four copies in flight (with
-// eight the whole eviction takes 105 us instead of 76).  Sources lie at or above `keep`, destinations below it, so moves never overlap.  Bound by
-// HBM and the latency of rows of 256 bytes in random places: 230,000 rows of 512 bytes in and out in about 45 us.
+// statistics, then the warp copies the key and value rows of all of them, 16 bytes a lane with four copies in flight.
+// Sources lie at or above `keep`, destinations below it, so moves never overlap.  Bound by HBM and the latency of rows in
+// random places: 226,000 moves of two 256-byte rows, in and out, in 41 us (5.6 TB/s).  The whole eviction then takes 69 us; 102
+// with eight copies in flight, 91 with seven CTAs an SM (more spills than the 28 bytes of six), 76 with four.  The same on E4M3
+// pages, whose scale bytes are moved one by one: 56 us for a floor of 21; E2M1 49 us for 12.
 __global__ void __launch_bounds__(kThreads, 6)
 evict_move_kernel(const Cache c, const Table table, const EvictArgs a, int row_bytes_log2, int scale_bytes, int per_warp) {
   wait_for_previous();
@@ -757,8 +759,9 @@ int mxq_paged_evict(const mxq_paged_cache *cache, int64_t batch, const int32_t *
   a.status = status;
   const Table t{page_table, table_stride, table_width};
   cudaStream_t st = (cudaStream_t)stream;
-  // Clusters of up to 8 CTAs share a long row's slots as long as there are fewer CTAs than SMs: 64 rows of 16384 slots 76 us
-  // with clusters of 4, 78 without (whole eviction); 8 rows of 1500 slots 15 us when shared by 2, 12 when not.
+  // Clusters of up to 8 CTAs share a long row's slots as long as there are fewer CTAs than SMs: 64 rows of 16384 slots 77 us
+  // with clusters of 4, 81 without (whole eviction), one such row 20.5 and 24.9; 8 rows of 1500 slots 14.4 us when shared by 2,
+  // 12.4 when not.
   int cluster = 1;
   while (cluster < 8 && width / cluster > kSlotsPerCta && rows * cluster < gemm::sm_count()) cluster *= 2;
   static std::atomic<bool> set_up[64];  // the kernel's shared memory limit has been raised on this device
@@ -779,8 +782,8 @@ int mxq_paged_evict(const mxq_paged_cache *cache, int64_t batch, const int32_t *
   if (rc != MXQ_OK || most == 0) return rc;
   const int row_bytes = row_bytes_of(cache->format, cache->head_dim);
   const int scale_bytes = cache->format == MXQ_CACHE_BF16 ? 0 : cache->head_dim / 32;
-  // Moves a warp looks up at once: 8 (8 x 16384 slots halved: 69 us; with 32, 76), or 4 so that there is work for four
-  // warps on every SM.
+  // Moves a warp looks up at once: 8 (8 x 12000 to 16384 slots halved: 69 us; with 32, 75), or 4 so that there is work for four
+  // warps on every SM (8 rows of 300 slots halved: 10.3 us; with 8, 11.7).
   int per_warp = 8;
   while (per_warp > 4 && rows * most < (int64_t)gemm::sm_count() * 4 * per_warp) per_warp /= 2;
   const int64_t per_cta = kThreads / 32 * per_warp;

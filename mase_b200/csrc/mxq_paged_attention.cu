@@ -9,18 +9,20 @@
 // The order of the summed index of a product is free, and so is the order of the rows of O^T, so a lane's operands are
 // pieces of up to 16 contiguous bytes of a row (four lanes share a key row, eight lanes a value row) and nothing is
 // transposed in memory; Q^T and the output follow the same permutation.  Tiles reach shared memory by asynchronous copies
-// in address order: with every lane copying its own operand pieces the same bytes arrived at 3.9 TB/s instead of 6.7.
+// in address order: a kernel of such copies and nothing else moves 6.7 TB/s, one whose lanes copy their own operand pieces 3.9.
 //
 // Codes become bf16 in registers: sign, exponent and fraction fields are moved to the bf16 positions with masks and
 // shifts and the result is multiplied by one power of two (block scale times the difference of the exponent biases).
 // Every value of every format has at most 8 significant bits, so this is exact, subnormal codes included.  bf16 queries
 // are exact operands too; fp32 queries are split into three bf16 terms.  Probabilities are fp32 and enter the second
-// product as two (fp32 queries: three) bf16 terms, 16 (24) significant bits; scores, maxima, sums and O^T are fp32.
+// product as two (fp32 queries: three) bf16 terms, 16 (24) significant bits, where the result keeps 8 (24); scores, maxima, sums
+// and O^T are fp32.
 //
 // Bound: HBM in principle (2 g multiply-adds per cached byte of a group of g query heads), in practice the instructions
 // that make bf16 of codes: 550 to 600 a tile of 16 x 128 one-byte codes, about 300 of them conversions; issue slots 63 % and the
-// logic unit 55 % busy.  Measured: 2 x 131072 tokens, 8 heads of 128, MXINT8: 107 us, 4.6 TB/s; 32 sequences of up to 8192,
-// E4M3: 69 us, 4.1 TB/s; bf16 pages, 16 x 2049 x 32 heads of 64: 37 us, 5.0 TB/s; copies alone reach 5.8 TB/s.
+// logic unit 55 % busy.  Measured (graph replays, join kernel included): sequences of 100001 and 131072 tokens, 8 heads of 128,
+// MXINT8: 105 us, 4.7 TB/s (with the copies alone 84 us, 5.8 TB/s); 32 sequences of 1 to 8192, E4M3: 70 us, 4.1 TB/s; bf16 pages,
+// 16 sequences of 777 to 2049, 32 heads of 64: 40 us, 4.6 TB/s.
 
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -39,8 +41,9 @@ namespace paged {
 constexpr int kWarps = 4;
 constexpr int kTile = 16;                // cached tokens of a warp's tile
 constexpr int kUnit = kWarps * kTile;    // tokens that a CTA takes at a time: the grain of the split
-constexpr int kRowCost = 2;              // units that a row counts for beyond its tokens: 1 / 2 / 4 made 84 / 78 / 80 us of
-                                         // 32 ragged sequences of up to 8192 tokens
+constexpr int kRowCost = 2;              // units that a row counts for beyond its tokens, 1 / 2 / 4: 32 sequences of 1 to 8192
+                                         // tokens 75 / 70 / 68 us, 64 of 1 to 100 tokens 16.4 / 16.4 / 18.4, 16 of 777 to
+                                         // 2049 in bf16 pages 40.3 / 39.8 / 40.6, append and 16 of 100 to 1023 18.5 / 20.5 / 19.8
 __host__ __device__ constexpr int finish_threads(int w) { return w > 4 ? 32 * w : 128; }
 
 struct AttnArgs {
@@ -138,7 +141,7 @@ struct Shape {
   static __host__ __device__ constexpr int value_turn(int i) {
     return kRow == 128 ? ((i >> 8) & 3) << 5 : (kRow == 256 ? ((i >> 9) & 3) << 5 : (kRow == 512 ? ((i >> 10) & 3) << 5 : 0));
   }
-  static constexpr int kStages = kRow <= 64 ? 4 : 2;  // three for rows of 128 bytes: 109 us against 107 (2 x 131072 MXINT8)
+  static constexpr int kStages = kRow <= 64 ? 4 : 2;  // three for rows of 128 bytes: 106 us against 105 (100001 + 131072 MXINT8)
 };
 // element (0 .. D-1) that half `half` of pair i of key word w of piece c of lane t holds
 template <int kFormat, int D>
@@ -509,7 +512,7 @@ __device__ __forceinline__ bool any_rare(uint32_t w, int bits) {
   }
 }
 
-// Three CTAs per SM where the registers would allow two: 107 us on 2 x 131072 MXINT8 tokens; four spill, 114 us.
+// Three CTAs per SM where the registers would allow two: 105 us on 100001 + 131072 MXINT8 tokens; two 119; four spill, 111.
 template <typename T, int kFormat, int D, int NT>
 __global__ void __launch_bounds__(kWarps * 32, Elem<T>::kBf16 && D == 128 && NT == 1 ? 3 : 1)
 attention_kernel(const Cache c, const Table table, const AttnArgs a) {
@@ -759,6 +762,9 @@ attention_kernel(const Cache c, const Table table, const AttnArgs a) {
 
 // Joins the parts of the rows that CTAs share, and adds the softmax weights of every token to the caller's statistics:
 //   weights[b, head, j] += sum over the group of exp(s_j - m) / l.
+// Without weights bound by latency: 8 to 9 us by itself, of which the launch during the attention kernel hides some.  With them,
+// 8 sequences of 3000 to 8192 tokens, 8 x 4 heads of 128, E4M3: 18 us for 12 MB, behind an attention kernel that takes 28 us
+// with the scores written and 26 without; the two calls take 43 and 33 us.
 // grid: (x, heads, batch): the x CTAs take the heads of the group in turn, W warps a head, and their threads the tokens.
 // Before the wait only what the attention kernel does not write is read: its CTAs let this kernel start after their own
 // wait, so everything before it in the stream has finished.
@@ -878,7 +884,7 @@ finish_kernel(const AttnArgs a, int heads, int tile_heads, int dim) {
 }
 
 // Query heads in tiles of 8, or of 16 for bf16 queries of more than 8 heads a group and head_dim <= 128 (larger ones do
-// not fit the registers): 16 heads a group over 8 x 8192 E4M3 tokens of 8 heads of 128 take 52 us in one tile, 64 us in two.
+// not fit the registers): 16 heads a group over 8 x 8192 E4M3 tokens of 8 heads of 128 take 55 us in one tile, 67 us in two.
 static int tiles_per_row(int dtype, int dim, int64_t group) { return dtype == MXQ_BF16 && group > 8 && dim <= 128 ? 2 : 1; }
 constexpr int kMostPerSm = 8;  // CTAs of the attention kernel on one SM, at most
 
@@ -1040,9 +1046,9 @@ int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, 
   rc = dtype == MXQ_BF16 ? launch_attention<__nv_bfloat16>(cache->format, dim, c, t, a, nt, most_ctas, st)
                          : launch_attention<float>(cache->format, dim, c, t, a, nt, most_ctas, st);
   if (rc != MXQ_OK || (!parts && !weights)) return rc;
-  // Warps for a head: one where rows are shared by few CTAs (64 sequences, 512 rows: 77 us against 89 with four), four or
-  // sixteen where they are shared by many (one row of 40000
-  // tokens in 444 parts: 21 us with sixteen, 77 with one; 16 rows of 28 parts: 105 us with four, 108 with one).
+  // Warps for a head: one where rows are shared by few CTAs (64 sequences, 512 rows: 80 us against 88 with four), four or
+  // sixteen where they are shared by many (one row of 40000 tokens in 444 parts: 23 us with sixteen, 33 with four, 94 with
+  // one; 16 rows of 28 parts: 104 us with four, 109 with one).
   const int64_t per_row = a.ctas / (batch * c.heads * a.head_tiles);
   const int w_head = per_row >= 64 ? 16 : (per_row >= 8 ? 4 : 1), threads = finish_threads(w_head);
   const int64_t at_once = threads / 32 / w_head;
