@@ -449,7 +449,8 @@ int mxq_paged_gather(const mxq_paged_cache *cache, void *key, void *value, int d
  * contiguous and 16-byte aligned.  q_heads is a multiple of heads: query heads h * g .. h * g + g - 1 read key/value head h.
  * weights (optional, fp32 [batch, heads, weights_width] contiguous): weights[b, h, j] += sum of softmax(s)_j over the
  * query heads of h.  workspace: 16-byte aligned, at least mxq_paged_attention_workspace_bytes(...) bytes, not shared with
- * a call that may run at the same time. */
+ * a call that may run at the same time; with weights 4 bytes a query head and slot of the table are part of it, so pass no more
+ * columns of the table (table_width) than the weights cover. */
 int64_t mxq_paged_attention_workspace_bytes(const mxq_paged_cache *cache, int64_t batch, int64_t q_heads,
                                             int64_t table_width, int with_weights);
 int mxq_paged_attention(const mxq_paged_cache *cache, const void *q, void *out, int dtype, int64_t batch, int64_t q_heads,
