@@ -480,6 +480,8 @@ class PagedKVState:
 
     def refresh(self) -> None:
         """Set max_length to the largest length now.  Reads the lengths back: not while a graph is captured."""
+        if self._capturing():
+            raise RuntimeError("PagedKVState.refresh reads the lengths back: call it before the capture")
         self.max_length = int(self.lengths.max()) if self.lengths.numel() else 0
 
     def _check_room(self, tokens: int) -> None:
@@ -490,7 +492,8 @@ class PagedKVState:
             after = self.lengths + (tokens if self.counts is None else self.counts)
             if after.numel() == 0 or int(after.max()) <= self.capacity:
                 return
-        raise ValueError(f"{self.max_length} + {tokens} tokens do not fit a page table of {self.capacity}")
+        raise ValueError(f"{self.max_length} + {tokens} tokens do not fit a page table of {self.capacity}"
+                         + (" (refresh() before the capture goes by the lengths)" if self._capturing() else ""))
 
     def lengths_after(self, tokens: int) -> Tensor:
         """The lengths once the forward's tokens are cached.  Added up by every call: a sum that is kept would not be part

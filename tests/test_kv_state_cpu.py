@@ -229,3 +229,15 @@ def test_page_tables_of_one_column_have_no_column_stride():
     assert _check_table(cache, wide[:1, ::8].t(), i32([1])) == 1
     with pytest.raises(ValueError, match="contiguous rows"):
         _check_table(cache, wide[:, ::2], i32([1, 2, 3]))
+
+
+def test_a_capture_cannot_look_at_the_lengths(monkeypatch):
+    state = make_state(lengths=[9, 5])
+    state.max_length = 60  # padding
+    with monkeypatch.context() as m:
+        m.setattr(state, "_capturing", lambda: True)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            state.refresh()
+        with pytest.raises(ValueError, match="do not fit.*before the capture"):
+            state.lengths_after(5)
+    assert state.lengths_after(5).tolist() == [14, 10] and state.max_length == 9
