@@ -435,9 +435,8 @@ class PagedKVState:
     the padded number of tokens to it; `refresh()` makes it the largest length again, which the room check does by itself
     before it refuses, and every forward on dense tensors once `advance` or `evict` has been captured into a graph.  A
     captured forward on dense tensors has them as long as they were at its capture: a replay with longer sequences is
-    reported by `check_status()`.  `lengths`, `next_position` and the tensors of `weights`
-    and `positions` are updated in place.  There is no backward pass: run the model under torch.no_grad() or
-    torch.inference_mode()."""
+    reported by `check_status()`.  `lengths`, `next_position` and the tensors of `weights` and `positions` are updated in
+    place.  There is no backward pass: run the model under torch.no_grad() or torch.inference_mode()."""
 
     def __init__(self, caches: list[PagedKVCache], page_table: Tensor, lengths: Tensor | None = None,
                  max_length: int | None = None, track: bool = False):
